@@ -101,6 +101,7 @@ extern "C" {
 /* bits of the optional device status word (PdDecodeArgs.status) */
 #define PD_DEV_BAD_BLOCK 1u   /* a block-table entry was outside [0, num_blocks): page skipped */
 #define PD_DEV_TIMEOUT 2u     /* a bounded wait inside a kernel gave up                        */
+#define PD_DEV_NO_BLOCKS 4u   /* pd_plan_step: a request's pages did not fit (pool or table row) */
 
 /*
  * Arguments of one decode step.  Replaces the argument list of paged_decode_triton
@@ -328,6 +329,110 @@ PD_API int pd_selftest_bounded_wait(uint32_t* status, uint64_t limit_ns, void* s
 /* Stores this step's keys and values into their cache slots, quantising to the cache's
  * element type with the reference's rules, bit for bit (see PdCacheWriteArgs). */
 PD_API int pd_cache_write(const PdCacheWriteArgs* args);
+
+/* Arguments of attention over the paged cache for more than pd_decode does: many new tokens per
+ * request (prompts, chunks of prompts, drafted tokens), and differential attention.
+ *
+ * The new tokens of all requests lie one behind another: request b owns the rows
+ * [query_start[b], query_start[b + 1]) of q and out, and they are the LAST tokens of its
+ * seq_lens[b] cached tokens (write them with pd_cache_write first).  The token at position p of a
+ * request attends to its keys 0 .. p.  Rows of q beyond query_start[batch] belong to nobody: their
+ * rows of out are left as they were.  A row whose position is below zero (more query rows than
+ * cached tokens) attends to nothing and gives zeros.
+ *
+ * maps = 1: out[t, h] = softmax(q[t, h] K^T * sm_scale) V.
+ * maps = 2 (differential): kv heads 2j and 2j + 1 are the two keys of pair j and their value rows,
+ * side by side, its value of 2 * head_dim; q[t, h, 0] and q[t, h, 1] are the queries of the two
+ * maps of query pair h, num_q_heads / 2 pairs in all, num_q_heads / num_kv_heads of them to a kv
+ * pair:
+ *   x = softmax(q[t, h, 0] K1^T * sm_scale) V - lam[t, h] * softmax(q[t, h, 1] K2^T * sm_scale) V
+ *   out[t, h] = norm ? x * rsqrt(mean(x^2) + eps) * norm_weight * out_scale : x * out_scale
+ * The scores, the softmax, both sums and the norm are held in 32 bits; the probabilities are
+ * rounded to q's type for the product with V by the kernels that use the matrix units.
+ *
+ * Keys and values of 8-bit pages are stored * scale, unrounded.  A block id outside the pool sets
+ * PD_DEV_BAD_BLOCK and its tokens are left out. */
+typedef struct PdPrefillArgs {
+  const void* q;   /* io_dtype, head_dim contiguous; strides: row, query head (maps = 2: query pair), map */
+  void* out;       /* io_dtype, [rows, num_q_heads, head_dim], or [rows, num_q_heads / 2, 2 * head_dim] */
+  int64_t q_stride_t, q_stride_h, q_stride_m;
+  int64_t out_stride_t, out_stride_h;
+  const void* k_cache;   /* cache side: as in PdDecodeArgs */
+  const void* v_cache;
+  int64_t kv_stride_block, kv_stride_token, kv_stride_head;
+  const void* k_scale;
+  const void* v_scale;
+  int64_t scale_stride_block, scale_stride_token;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* seq_lens;     /* [batch] tokens in the cache, the new ones among them */
+  const int32_t* query_start;  /* [batch + 1] ascending; pd_diff_decode: NULL (row b is request b's) */
+  int32_t num_rows;            /* rows of q and out */
+  int32_t batch, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq;
+  int32_t kv_dtype, io_dtype;
+  float sm_scale;
+  int32_t maps;                /* 1, or 2: differential */
+  const float* lam;            /* maps = 2: device, strides below (0 broadcasts); NULL: lam_value */
+  int64_t lam_stride_t, lam_stride_h;
+  float lam_value;
+  const float* norm_weight;    /* [2 * head_dim] dense, or NULL: ones */
+  float eps, out_scale;
+  int32_t norm;                /* 0: no norm */
+  int32_t kernel;              /* PD_KERNEL_*: STREAM is the one on the matrix units */
+  int32_t sm_count;            /* 0 = query the current device */
+  int32_t max_seq_len;         /* optional bound on seq_lens (0 = unknown): refines the split count */
+  void* workspace;             /* 256-byte aligned, pd_prefill_workspace_bytes() bytes */
+  uint64_t workspace_bytes;
+  uint32_t* status;            /* optional device word, OR-ed with PD_DEV_* bits; caller zeroes it */
+  void* stream;
+} PdPrefillArgs;
+
+/* Causal attention of many new tokens per request over the paged cache (maps = 1 or 2). */
+PD_API int pd_prefill(const PdPrefillArgs* args);
+
+/* Differential attention of ONE new token per request (maps = 2, query_start NULL, num_rows =
+ * batch): row b attends to all seq_lens[b] tokens. */
+PD_API int pd_diff_decode(const PdPrefillArgs* args);
+
+/* Scratch and kernel choice of the two (by query_start being NULL), as pd_workspace_bytes and
+ * pd_select_kernel are for pd_decode. */
+PD_API int pd_prefill_workspace_bytes(const PdPrefillArgs* args, uint64_t* bytes);
+PD_API int pd_prefill_select_kernel(const PdPrefillArgs* args);
+
+/* Block tables, slot map, positions and lengths of one step, from request lengths, on the device.
+ *
+ * Request b has context_lens[b] tokens in the cache and gets new_tokens[b] more (negative values
+ * count as zero).  The pages it lacks are taken from the free list, a stack whose top is
+ * free_blocks[num_free - 1], in request order, and entered into its block-table row behind the
+ * pages it has.  A request is served if its row has room for all its pages and the free list
+ * holds the pages of all such requests up to and including it; one that needs no page always is.
+ * A request that is not served keeps its length and its row, its tokens get slot -1, and
+ * PD_DEV_NO_BLOCKS is raised.
+ *
+ * Outputs: slot_mapping[t] = block * block_size + offset of new token t (request after request),
+ * positions[t] its position in its request; entries behind the last new token are -1 and 0.
+ * query_start[b] = new tokens before request b, query_start[batch] = all; seq_lens[b]; num_free_out.
+ * seq_lens may be context_lens and num_free_out may be num_free (nothing is written before all of
+ * both has been read); no other overlap is allowed. */
+typedef struct PdPlanArgs {
+  int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* context_lens;   /* [batch] */
+  const int32_t* new_tokens;     /* [batch] */
+  const int32_t* free_blocks;    /* [free_capacity] */
+  const int32_t* num_free;       /* [1] */
+  int64_t* slot_mapping;         /* [num_tokens] */
+  int64_t* positions;            /* [num_tokens] */
+  int32_t* query_start;          /* [batch + 1] */
+  int32_t* seq_lens;             /* [batch] */
+  int32_t* num_free_out;         /* [1] */
+  int32_t batch, max_blocks_per_seq, block_size, free_capacity, num_tokens;
+  uint32_t* status;              /* optional device word */
+  void* stream;
+} PdPlanArgs;
+
+/* One launch; at most 8192 requests, fewer than 2^31 new tokens in all. */
+PD_API int pd_plan_step(const PdPlanArgs* args);
 
 /*
  * pd_decode for callers that have no scratch memory to give and may not allocate any.  It has

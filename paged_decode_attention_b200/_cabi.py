@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 
 import torch
 
@@ -24,6 +25,7 @@ IO_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
 DEV_BAD_BLOCK = 1
 DEV_TIMEOUT = 2
+DEV_NO_BLOCKS = 4
 
 _c_i32, _c_i64, _c_u64, _c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_void_p
 
@@ -90,6 +92,54 @@ class PdExchangeArgs(ctypes.Structure):
     ]
 
 
+class PdPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _c_vp), ("out", _c_vp),
+        ("q_stride_t", _c_i64), ("q_stride_h", _c_i64), ("q_stride_m", _c_i64),
+        ("out_stride_t", _c_i64), ("out_stride_h", _c_i64),
+        ("k_cache", _c_vp), ("v_cache", _c_vp),
+        ("kv_stride_block", _c_i64), ("kv_stride_token", _c_i64), ("kv_stride_head", _c_i64),
+        ("k_scale", _c_vp), ("v_scale", _c_vp),
+        ("scale_stride_block", _c_i64), ("scale_stride_token", _c_i64),
+        ("block_table", _c_vp), ("block_table_stride", _c_i64),
+        ("seq_lens", _c_vp), ("query_start", _c_vp),
+        ("num_rows", _c_i32),
+        ("batch", _c_i32), ("num_q_heads", _c_i32), ("num_kv_heads", _c_i32), ("head_dim", _c_i32),
+        ("block_size", _c_i32), ("num_blocks", _c_i32), ("max_blocks_per_seq", _c_i32),
+        ("kv_dtype", _c_i32), ("io_dtype", _c_i32),
+        ("sm_scale", ctypes.c_float),
+        ("maps", _c_i32),
+        ("lam", _c_vp), ("lam_stride_t", _c_i64), ("lam_stride_h", _c_i64), ("lam_value", ctypes.c_float),
+        ("norm_weight", _c_vp), ("eps", ctypes.c_float), ("out_scale", ctypes.c_float), ("norm", _c_i32),
+        ("kernel", _c_i32), ("sm_count", _c_i32), ("max_seq_len", _c_i32),
+        ("workspace", _c_vp), ("workspace_bytes", _c_u64),
+        ("status", _c_vp), ("stream", _c_vp),
+    ]
+
+
+class PdPlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("block_table", _c_vp), ("block_table_stride", _c_i64),
+        ("context_lens", _c_vp), ("new_tokens", _c_vp), ("free_blocks", _c_vp), ("num_free", _c_vp),
+        ("slot_mapping", _c_vp), ("positions", _c_vp), ("query_start", _c_vp), ("seq_lens", _c_vp),
+        ("num_free_out", _c_vp),
+        ("batch", _c_i32), ("max_blocks_per_seq", _c_i32), ("block_size", _c_i32), ("free_capacity", _c_i32),
+        ("num_tokens", _c_i32),
+        ("status", _c_vp), ("stream", _c_vp),
+    ]
+
+
+_PACK_CODE = {_c_vp: "P", _c_i64: "q", _c_i32: "i", _c_u64: "Q", ctypes.c_float: "f", ctypes.c_uint32: "I"}
+
+
+def packer(struct_type):
+    """``struct.Struct`` of a ctypes structure with native alignment: one ``pack`` call makes an
+    argument block several times faster than forty attribute assignments."""
+    s = struct.Struct("@" + "".join(_PACK_CODE[t] for _, t in struct_type._fields_) + "0P")
+    assert s.size == ctypes.sizeof(struct_type)
+    return s
+
+
 class PdGatherArgs(ctypes.Structure):
     _fields_ = [("cache", ctypes.POINTER(PdDecodeArgs)), ("k_dense", _c_vp), ("v_dense", _c_vp),
                 ("s_max", _c_i32)]
@@ -98,7 +148,8 @@ class PdGatherArgs(ctypes.Structure):
 EXPORTS = ("pd_abi_version", "pd_status_string", "pd_decode", "pd_decode_host",
            "pd_workspace_bytes", "pd_select_kernel", "pd_pick_num_splits", "pd_merge", "pd_gather",
            "pd_decode_static", "pd_cache_write", "pd_selftest_bounded_wait", "pd_exchange_bytes",
-           "pd_exchange_step", "pd_exchange_part_offset", "pd_decode_exchange", "pd_counter_bytes")
+           "pd_exchange_step", "pd_exchange_part_offset", "pd_decode_exchange", "pd_counter_bytes",
+           "pd_prefill", "pd_diff_decode", "pd_prefill_workspace_bytes", "pd_prefill_select_kernel", "pd_plan_step")
 
 FLAG_COUNTERS_ZERO = 1
 FLAG_EQUAL_TILE_SHARES = 2
@@ -163,6 +214,12 @@ def load() -> ctypes.CDLL:
     lib.pd_selftest_bounded_wait.argtypes = [_c_vp, _c_u64, _c_vp]
     lib.pd_cache_write.restype = ctypes.c_int
     lib.pd_cache_write.argtypes = [ctypes.POINTER(PdCacheWriteArgs)]
+    # these take packed argument blocks (see packer)
+    for name in ("pd_prefill", "pd_diff_decode", "pd_prefill_select_kernel", "pd_plan_step"):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [ctypes.c_char_p]
+    lib.pd_prefill_workspace_bytes.restype = ctypes.c_int
+    lib.pd_prefill_workspace_bytes.argtypes = [ctypes.c_char_p, ctypes.POINTER(_c_u64)]
     _lib = lib
     return lib
 

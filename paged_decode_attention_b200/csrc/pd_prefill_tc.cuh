@@ -1,0 +1,861 @@
+// Causal attention of many new tokens per request over the paged cache, on the fifth-generation
+// matrix units (pd_prefill with maps = 1 or 2).
+//
+// Mathematics.  For one kv head the rows (token, head of its group) of a request are packed into
+// tiles of 128; a tile walks the request's keys in blocks of 128 with the base-2 online softmax:
+//   S = Q K^T,  m' = max(m, max S),  P = 2^(S - m'),  l = l 2^(m - m') + sum P,  O = O 2^(m - m') + P V.
+// A CTA has two such tiles.  maps = 1: the two halves of 256 packed rows, against the same keys.
+// maps = 2: the SAME 128 rows with their two queries against the two keys of the pair, and one V of
+// 2 * head_dim columns; the epilogue subtracts, norms and stores.  A CTA holds at most 128 columns of
+// V: for head_dim 128 the two halves belong to a cluster of two CTAs, which exchange the rows'
+// sums of squares.
+//
+// Why so.  Per tile and block the matrix units take 128 * 128 * (D + DV) multiply-adds, 4096 a
+// cycle, and the special function units 128 * 128 exponentials, 16 a cycle: 1024 cycles of each at
+// D = DV = 128.  Neither may wait for the other, hence the two tiles: while one tile's softmax runs
+// on its four warps, the matrix units work for the other.  A thread owns one row, so maximum and sum
+// need no exchange.  S and O stay in tensor memory (2 * (128 + DV) columns), P replaces S there as
+// 16-bit pairs and is read by the second product from tensor memory; shared memory holds Q and a
+// ring of K and V tiles that one warp fills by TMA, page by page, in the 128-byte swizzle.
+//
+// The maximum that P refers to may lag behind the true one by kLag (2^3 or 2^8 at most): O is then not
+// rescaled for every small rise.  It cancels in O / l; l and O are 32-bit.
+//
+// Few rows and long contexts: the key blocks are split over `splits` CTAs, each writes normalised
+// 32-bit rows and their log-sum-exp, and a second kernel joins them.
+//
+// 8-bit pages: four more warps read the pages, widen the elements exactly and store them in the
+// same swizzle; K's scales multiply S, V's scales multiply P (times 32, against fp16's subnormals),
+// so nothing is rounded on the way.
+//
+// Every wait is bounded; one that gives up raises PD_DEV_TIMEOUT and ends the CTA's loops.  Nobody
+// skips a barrier on that way, tensor memory is freed, and copies and products in flight are
+// awaited (bounded) first.
+#pragma once
+
+#include "pd_prefill.h"
+#include "pd_stream_kernel.cuh"
+
+namespace pd {
+
+constexpr int kTcBlock = 128;      // keys of one block, rows of one tile
+constexpr int kTcMetaRing = 16;    // blocks whose bad-page masks are kept
+constexpr int kTcSmem = 227 * 1024;
+
+template <int KV, int D, int MAPS, bool SCALED>
+struct TcCfg {
+  static constexpr bool WIDEN = !is_16bit(KV);             // 8-bit pages: converting warps instead of TMA
+  static constexpr bool BF16 = KV == PD_KV_BF16;
+  static constexpr int DV = MAPS == 2 ? 128 : D;           // columns of V in one CTA
+  static constexpr int SLICES = MAPS * D / DV;             // CTAs that share V's columns
+  static constexpr int VH = DV / D > 1 ? DV / D : 1;       // V heads side by side in the slice
+  static constexpr int NP = SCALED ? VH : 1;               // different P operands (one for each V head's scales)
+  static constexpr int KT = MAPS;                          // K tiles of one block
+  static constexpr int ROWS = MAPS == 2 ? 128 : 256;       // packed rows of one CTA
+  static constexpr int QTILE = 128 * D * 2;
+  static constexpr int SLOT = 128 * (D > DV ? D : DV) * 2;
+  static constexpr int SCALE_FLOATS = SCALED ? (KT + VH) * 128 : 0;  // of one block
+  static constexpr int SCALE_RING = 4;
+  static constexpr int FIXED = 1024 + 2 * QTILE + SCALE_RING * SCALE_FLOATS * 4 + 2048;
+  static constexpr int FIT = (kTcSmem - FIXED) / SLOT;
+  static constexpr int NSLOT = FIT > 8 ? 8 : FIT;
+  static constexpr int SMEM = FIXED + NSLOT * SLOT;
+  static constexpr int WARPS = WIDEN ? 14 : 10;            // softmax 0-3 and 4-7, loader 8, matrix units 9, widening 10-13
+  static constexpr int THREADS = WARPS * 32;
+  static_assert(NSLOT >= 3 && SMEM <= kTcSmem, "shared memory");
+};
+
+struct TcParams {
+  PrefillParams a;
+  int32_t tiles, heads, splits;  // grid: splits x tiles x heads (x slices)
+  int32_t box_tokens;            // tokens of one TMA box
+  float* part_o;                 // splits > 1: [split][row][head, map][columns of V in all], log-sum-exps
+  float* part_lse;
+};
+
+// ---- tcgen05 wrappers ----------------------------------------------------------------------------
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (128 x N, f32, tensor memory) (+)= A (128 x 16) * B (16 x N); A and B by shared-memory descriptors
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0)
+      : "memory");
+}
+// the same with A in tensor memory (16-bit pairs)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0)
+      : "memory");
+}
+#define PD_R8(x, i) "=r"((x)[i]), "=r"((x)[i + 1]), "=r"((x)[i + 2]), "=r"((x)[i + 3]), "=r"((x)[i + 4]), \
+                    "=r"((x)[i + 5]), "=r"((x)[i + 6]), "=r"((x)[i + 7])
+#define PD_I8(x, i) "r"((x)[i]), "r"((x)[i + 1]), "r"((x)[i + 2]), "r"((x)[i + 3]), "r"((x)[i + 4]), \
+                    "r"((x)[i + 5]), "r"((x)[i + 6]), "r"((x)[i + 7])
+// 32 columns of the warp's 32 lanes: thread = lane, register = column
+__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* x) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : PD_R8(x, 0), PD_R8(x, 8), PD_R8(x, 16), PD_R8(x, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(addr), PD_I8(x, 0), PD_I8(x, 8), PD_I8(x, 16), PD_I8(x, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* x) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(addr), PD_I8(x, 0), PD_I8(x, 8)
+      : "memory");
+}
+
+// Shared-memory operand descriptor in the 128-byte swizzle: 8-row groups 1024 bytes apart.  K-major
+// tiles have 64 elements of the inner dimension per row, the leading offset is not used; MN-major ones
+// (V) have 64 columns per row and find the next 64 columns `lead` bytes on.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((lead >> 4) & 0x3fffu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor: f32 accumulators, f16 or bf16 operands, M = 128, N columns, B MN-major or K-major.
+__host__ __device__ constexpr uint32_t tc_idesc(bool bf16, int n, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_half2(lo, hi);
+  }
+}
+
+// What a CTA works on.
+struct TcTile {
+  int request, row0, count;  // first packed row (within the request) and packed rows, at most ROWS
+  int first_token;           // row of q of the request's first token
+  int tokens, len;           // new tokens and cached tokens of the request
+};
+
+// The tile with number i: request b's tiles begin at floor(query_start[b] * group / ROWS) + b, which leaves
+// room for ceil(tokens * group / ROWS) of them.  Found by one warp, 32 probes at a time.
+__device__ __forceinline__ bool tc_find_tile(const PrefillParams& a, int rows_per_tile, int i, int lane, TcTile& t) {
+  const Params& p = a.p;
+  const int64_t group = p.group;
+  int lo = 0, n = p.batch;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lane * step;
+    const bool before = at < n && (int64_t)__ldg(a.starts + lo + at) * group / rows_per_tile + lo + at <= i;
+    const int k = max(__popc(__ballot_sync(0xffffffffu, before)) - 1, 0);
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  const int start = __ldg(a.starts + lo);
+  int tokens = __ldg(a.starts + lo + 1) - start;
+  if (start < 0 || start >= a.rows || tokens <= 0) return false;
+  tokens = min(tokens, a.rows - start);
+  const int64_t local = i - ((int64_t)start * group / rows_per_tile + lo);
+  if (local < 0 || local * rows_per_tile >= (int64_t)tokens * group) return false;
+  t.request = lo;
+  t.row0 = (int)(local * rows_per_tile);
+  t.count = (int)min((int64_t)rows_per_tile, (int64_t)tokens * group - t.row0);
+  t.first_token = start;
+  t.tokens = tokens;
+  t.len = clamp_len(p, lo);
+  return true;
+}
+
+// Keys that packed row r of the request sees.
+__device__ __forceinline__ int tc_limit(const TcTile& t, int r, int group) {
+  const int n = t.len - t.tokens + r / group + 1;
+  return n < 0 ? 0 : n;  // r is the request's: at most t.len
+}
+
+template <int KV, int D, int MAPS, bool SCALED>
+__global__ void __launch_bounds__(TcCfg<KV, D, MAPS, SCALED>::THREADS, 1)
+tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v) {
+  using C = TcCfg<KV, D, MAPS, SCALED>;
+  constexpr unsigned kFull = 0xffffffffu;
+  constexpr float kLag = SCALED ? 3.f : 8.f;    // P is at most 2^kLag (times a V scale and 32: below fp16's range up to scales of 255)
+  constexpr float kBoost = SCALED ? 32.f : 1.f;
+  const PrefillParams& a = tp.a;
+  const Params& p = a.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t ring0 = base, q0 = base + C::NSLOT * C::SLOT;
+  float* scales = reinterpret_cast<float*>(smem + C::NSLOT * C::SLOT + 2 * C::QTILE);
+  uint8_t* misc = smem + C::NSLOT * C::SLOT + 2 * C::QTILE + C::SCALE_RING * C::SCALE_FLOATS * 4;
+  volatile int* meta = reinterpret_cast<volatile int*>(misc);               // bad 16-token pieces of a block
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 64);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc + 68);
+  TcTile* tile_sh = reinterpret_cast<TcTile*>(misc + 96);
+  volatile int* have_tile = reinterpret_cast<volatile int*>(misc + 128);
+  const uint32_t bars = smem_u32(misc) + 256;
+  const uint32_t full0 = bars, empty0 = bars + 64, s_full = bars + 128, p_full = bars + 144, o_done = bars + 160,
+                 q_full = bars + 176, tail_bar = bars + 184, drain_bar = bars + 192;
+  float* squares = reinterpret_cast<float*>(misc + 512);  // [128] of the peer's half rows
+  static_assert(512 + 128 * 4 <= 2048, "misc area");
+
+  // ---- which tile ------------------------------------------------------------------------------
+  const int slice = C::SLICES == 1 ? 0 : blockIdx.x % C::SLICES;
+  int work = blockIdx.x / C::SLICES;
+  const int head = work % tp.heads;  // kv head, or kv pair
+  work /= tp.heads;
+  const int tile_no = tp.tiles - 1 - work % tp.tiles;  // a prompt's last tiles are its longest: they go first
+  const int split = work / tp.tiles;
+  if (warp == 0) {
+    TcTile t;
+    const bool ok = tc_find_tile(a, C::ROWS, tile_no, lane, t);
+    if (lane == 0) {
+      *have_tile = ok ? 1 : 0;
+      if (ok) *tile_sh = t;
+      *abort_flag = 0;
+      for (int i = 0; i < kTcMetaRing; ++i) meta[i] = 0;
+    }
+  }
+  if (warp == 8 && lane == 0) {
+    for (int s = 0; s < C::NSLOT; ++s) {
+      mbar_init(full0 + 8 * s, C::WIDEN ? 128 : 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full + 8 * t, 1);
+      mbar_init(p_full + 8 * t, 128);
+      mbar_init(o_done + 8 * t, 1);
+    }
+    mbar_init(q_full, 256);
+    mbar_init(tail_bar, 1);
+    mbar_init(drain_bar, 1);
+    fence_barrier_init();
+    fence_proxy_async();
+    if constexpr (!C::WIDEN) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&tm_k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&tm_v) : "memory");
+    }
+  }
+  __syncthreads();
+  if (!*have_tile) return;  // the whole cluster has the same tile: nobody waits for this CTA
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((const void*)tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const TcTile tile = *tile_sh;
+
+  // ---- the tiles' rows and key blocks ----------------------------------------------------------------
+  // maps = 1: tile t has the packed rows 128 t ..; maps = 2: both tiles have the same rows
+  int rows_of[2], begin[2], end[2];  // rows, first and last + 1 key block
+  const int last_row = tile.row0 + tile.count - 1;
+  const int blocks = (tc_limit(tile, last_row, p.group) + kTcBlock - 1) / kTcBlock;  // of the longest row
+  const int chunk = (blocks + tp.splits - 1) / tp.splits;
+  const int j0 = min(split * chunk, blocks), j1 = min(j0 + chunk, blocks);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    rows_of[t] = MAPS == 2 ? tile.count : max(0, min(128, tile.count - 128 * t));
+    const int top = rows_of[t] ? tc_limit(tile, tile.row0 + (MAPS == 2 ? 0 : 128 * t) + rows_of[t] - 1, p.group) : 0;
+    begin[t] = j0;
+    end[t] = max(j0, min(j1, (top + kTcBlock - 1) / kTcBlock));
+  }
+  const int jend = max(end[0], end[1]);
+  const int kv_end = tc_limit(tile, last_row, p.group);  // keys from here on are zero in shared memory
+
+  // ================================ loader (16-bit pages) =============================================
+  if (warp == 8) {
+    if constexpr (!C::WIDEN) {
+      const int bt = tp.box_tokens, boxes = kTcBlock / bt;
+      int unit = 0;
+      bool tail_used = false;
+      // Unit order: K of the first block, then V of each block followed by K of the next.
+      const int nb = jend - j0;
+      const int units = nb > 0 ? nb * (C::KT + 1) : 0;
+      for (; unit < units; ++unit) {
+        // position in the cycle of V, K.. (the first block's K come ahead of it)
+        int j, k;  // block; K tile number or -1: V
+        if (unit < C::KT) {
+          j = j0;
+          k = unit;
+        } else {
+          const int u = unit - C::KT;
+          const int cyc = u / (C::KT + 1), in = u % (C::KT + 1);
+          j = j0 + cyc + (in ? 1 : 0);
+          k = in - 1;
+        }
+        const int st = unit % C::NSLOT;
+        int ok = 1;
+        const uint32_t dst = ring0 + st * C::SLOT;
+        const int token = j * kTcBlock + lane * bt;
+        int phys = p.num_blocks, off = 0, bad = 0;  // out of the map: zeros
+        if (lane < boxes && token < kv_end) {
+          const int page = token / p.page;
+          off = token - page * p.page;
+          const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
+          if ((unsigned)id < (unsigned)p.num_blocks) phys = id;
+          else {
+            if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
+            bad = ((1 << (bt / 16)) - 1) << (lane * bt / 16);
+          }
+        }
+        bad = __reduce_or_sync(kFull, (unsigned)bad);
+        // V rows from kv_end to the end of their box hold whatever the page holds: zero times that may be
+        // NaN, so they are cleared behind the copy
+        const int live = kv_end - j * kTcBlock;  // keys of the block that exist
+        const bool tail = k < 0 && live < kTcBlock && live % bt != 0;
+        if (lane == 0) {
+          ok = mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag) ? 1 : 0;
+          if (ok) {
+            meta[j & (kTcMetaRing - 1)] = bad;
+            mbar_arrive_expect_tx(tail ? tail_bar : full0 + 8 * st, 128 * 2 * (k < 0 ? C::DV : D));
+          }
+        }
+        if (!__shfl_sync(kFull, ok, 0)) break;
+        if (lane < boxes) {
+          const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
+          const uint32_t at = dst + lane * bt * 128;
+          if (k >= 0) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(at + c * (128 * 128), &tm_k, bar, c * 64, off, head * MAPS + k, phys);
+          } else {
+#pragma unroll
+            for (int c = 0; c < C::DV / 64; ++c) {
+              const int col = slice * C::DV + c * 64;  // column of the pair's (or head's) V
+              tma_load_4d(at + c * (128 * 128), &tm_v, bar, col % D, off, head * MAPS + col / D, phys);
+            }
+          }
+        }
+        __syncwarp();
+        if (tail) {
+          tail_used = true;
+          int landed = 1;
+          if (lane == 0) landed = mbar_wait(tail_bar, 0, p.status, abort_flag) ? 1 : 0;  // the one tail of this CTA
+          if (!__shfl_sync(kFull, landed, 0)) {
+            ++unit;
+            break;
+          }
+          const int to = (live / bt + 1) * bt;
+          for (int i = lane; i < (to - live) * (C::DV / 64) * 8; i += 32) {
+            const int r = live + i / 8 % (to - live), c = i / 8 / (to - live);
+            sts128(dst + c * (128 * 128) + r * 128 + (i & 7) * 16, make_uint4(0, 0, 0, 0));
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full0 + 8 * st);
+        }
+      }
+      if (*abort_flag && lane == 0) {  // copies still in flight get a bounded chance to land
+        for (int k = 1; k <= C::NSLOT && k <= unit; ++k)
+          mbar_wait_slow(full0 + 8 * ((unit - k) % C::NSLOT), (uint32_t)((unit - k) / C::NSLOT) & 1u, nullptr, abort_flag, false);
+        if (tail_used) mbar_wait_slow(tail_bar, 0, nullptr, abort_flag, false);
+      }
+    }
+  }
+  // ================================ widening warps (8-bit pages) =======================================
+  else if (warp >= 10) {
+    if constexpr (C::WIDEN) {
+      const int me = tid - 320;  // 0 .. 127
+      constexpr int kMaxChunk = (D > C::DV ? D : C::DV) / 16;  // 16-byte pieces of a row = pieces per thread and tile
+      const int nb = jend - j0;
+      const int units = nb > 0 ? nb * (C::KT + 1) : 0;
+      bool ok = true;
+      for (int unit = 0; unit < units && ok; ++unit) {
+        int j, k;
+        if (unit < C::KT) {
+          j = j0;
+          k = unit;
+        } else {
+          const int u = unit - C::KT;
+          const int cyc = u / (C::KT + 1), in = u % (C::KT + 1);
+          j = j0 + cyc + (in ? 1 : 0);
+          k = in - 1;
+        }
+        const int st = unit % C::NSLOT;
+        const uint32_t dst = ring0 + st * C::SLOT;
+        const int pieces = (k < 0 ? C::DV : D) / 16;  // of one row; a warp-wide load covers whole rows
+        uint4 x[kMaxChunk];
+#pragma unroll
+        for (int i = 0; i < kMaxChunk; ++i) {
+          x[i] = make_uint4(0, 0, 0, 0);
+          const int n = me + i * 128;
+          const int r = n / pieces, c = n % pieces;
+          const int token = j * kTcBlock + r;
+          if (i < pieces && token < kv_end) {
+            const int page = token / p.page;
+            const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
+            if ((unsigned)id < (unsigned)p.num_blocks) {
+              const int col = k < 0 ? slice * C::DV + c * 16 : c * 16;
+              const int64_t at = kv_row_offset(p, id, token - page * p.page, head * MAPS + (k < 0 ? col / D : k)) + col % D;
+              x[i] = __ldg(reinterpret_cast<const uint4*>((const char*)(k < 0 ? p.v : p.k) + at));
+            } else {
+              if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
+              atomicOr(const_cast<int*>(&meta[j & (kTcMetaRing - 1)]), 1 << (r / 16));
+            }
+          }
+        }
+        // the block's scales: one token a thread
+        float sc[SCALED ? C::VH : 1] = {};
+        if constexpr (SCALED) {
+          const int token = j * kTcBlock + me;
+          if (token < kv_end) {
+            const int page = token / p.page;
+            const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
+            if ((unsigned)id < (unsigned)p.num_blocks) {
+              if (k >= 0) {
+                sc[0] = __half2float(__ldg(p.k_scale + scale_offset(p, id, token - page * p.page, head * MAPS + k)));
+              } else {
+#pragma unroll
+                for (int z = 0; z < C::VH; ++z)
+                  sc[z] = kBoost * __half2float(__ldg(p.v_scale + scale_offset(p, id, token - page * p.page,
+                                                                               head * MAPS + (MAPS == 2 ? slice * C::DV / D + z : 0))));
+              }
+            }
+          }
+        }
+        ok = mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kMaxChunk; ++i) {
+          if (i >= pieces) continue;
+          const int n = me + i * 128;
+          const int r = n / pieces, c = n % pieces;
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t y = KV == PD_KV_I8 ? w[e] ^ 0x80808080u : w[e];
+            h[2 * e] = cvt_pair<KV>(y, false);
+            h[2 * e + 1] = cvt_pair<KV>(y, true);
+          }
+          if constexpr (KV == PD_KV_E5M2) {
+            // cvt_pair places bytes (0, 1) and (2, 3) above zero bytes, in order
+          }
+          const uint32_t row = dst + (c / 4) * (128 * 128) + r * 128;
+          const int ch = (2 * c) & 7;
+          // neighbours that share banks store their two halves in opposite order
+          const int flip = (c >> 2) & 1;
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            const int half = o ^ flip;
+            const uint4 y = half ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+            sts128(row + (((ch + half) ^ (r & 7)) << 4), y);
+          }
+        }
+        if constexpr (SCALED) {
+          float* at = scales + (j % C::SCALE_RING) * C::SCALE_FLOATS;
+          if (k >= 0) at[k * 128 + me] = sc[0];
+          else {
+#pragma unroll
+            for (int z = 0; z < C::VH; ++z) at[(C::KT + z) * 128 + me] = sc[z];
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(full0 + 8 * st);
+      }
+    }
+  }
+  // ================================ matrix units ======================================================
+  else if (warp == 9) {
+    if (lane == 0) {
+      constexpr uint32_t id_s = tc_idesc(C::BF16, 128, false);
+      constexpr uint32_t id_o = tc_idesc(C::BF16, C::DV / C::NP, true);
+      int unit = 0;
+      bool ok = true;
+      auto wait_unit = [&](int u) { return mbar_wait(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u, p.status, abort_flag); };
+      auto scores = [&](int t, uint32_t kslot) {  // S_t = Q_t K^T
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
+          tc_mma_ss(tmem + t * 128, tc_desc(q0 + t * C::QTILE + off, 0), tc_desc(kslot + off, 0), id_s, ks > 0);
+        }
+        tc_commit(s_full + 8 * t);
+      };
+      auto values = [&](int t, uint32_t vslot, bool first) {  // O_t (+)= P_t V
+#pragma unroll
+        for (int z = 0; z < C::NP; ++z) {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t pa = C::NP == 1 ? 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks % 2);
+            tc_mma_ts(tmem + 256 + t * 128 + z * 64, tmem + t * 128 + pa,
+                      tc_desc(vslot + z * (128 * 128) + ks * 2048, 128 * 128), id_o, !first || ks > 0);
+          }
+        }
+      };
+      if (jend > j0) {
+        ok = mbar_wait(q_full, 0, p.status, abort_flag);
+        // the first block's scores
+        if (ok) ok = wait_unit(0);
+        if (ok) {
+          tc_fence_after();
+          if (end[0] > j0) scores(0, ring0);
+          if constexpr (MAPS == 2) {
+            ok = wait_unit(1);
+            tc_fence_after();
+            if (ok) {
+              scores(1, ring0 + (1 % C::NSLOT) * C::SLOT);
+              tc_commit(empty0);
+              tc_commit(empty0 + 8);
+            }
+          } else {
+            if (end[1] > j0) scores(1, ring0);
+            tc_commit(empty0);
+          }
+        }
+        unit = C::KT;
+        for (int j = j0; j < jend && ok; ++j) {
+          const int vs = unit % C::NSLOT;
+          const bool more = j + 1 < jend;
+          bool have_v = false, have_k = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= end[t] || !ok) continue;
+            ok = mbar_wait(p_full + 8 * t, (uint32_t)(j - j0) & 1u, p.status, abort_flag);
+            if (ok && !have_v) ok = wait_unit(unit);
+            if (!ok) break;
+            have_v = true;
+            tc_fence_after();
+            values(t, ring0 + vs * C::SLOT, j == j0);
+            if (j + 1 < end[t]) {
+              const int ku = unit + 1 + (MAPS == 2 ? t : 0);
+              if (MAPS == 2 || !have_k) ok = wait_unit(ku);
+              if (!ok) break;
+              have_k = true;
+              tc_fence_after();
+              scores(t, ring0 + (ku % C::NSLOT) * C::SLOT);
+            } else {
+              tc_commit(o_done + 8 * t);
+            }
+          }
+          if (!ok) break;
+          // both tiles' products with these tiles are issued: their slots are free when they are done
+          tc_commit(empty0 + 8 * vs);
+          ++unit;
+          if (more) {
+#pragma unroll
+            for (int k = 0; k < C::KT; ++k) tc_commit(empty0 + 8 * ((unit + k) % C::NSLOT));
+            unit += C::KT;
+          }
+        }
+        if (!ok) {  // products in flight get a bounded chance to end before tensor memory is freed
+          tc_commit(drain_bar);
+          mbar_wait_slow(drain_bar, 0, nullptr, abort_flag, false);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  // ================================ softmax ============================================================
+  else {
+    const int t = warp >> 2;            // tile
+    const int me = tid & 127;           // row of the tile
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
+    const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
+    const int first_row = tile.row0 + (MAPS == 2 ? 0 : 128 * t);  // packed row of the tile's row 0
+    const int n_rows = rows_of[t];
+
+    // ---- Q into shared memory, 16 bytes at a time, in the 128-byte swizzle --------------------------
+    if (jend > j0) {
+      constexpr int CH = D / 8;  // pieces of a row
+#pragma unroll 4
+      for (int i = me; i < 128 * CH; i += 128) {
+        const int r = i / CH, c = i % CH;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < n_rows) {
+          const int pr = first_row + r;
+          const int tok = pr / p.group, g = pr - tok * p.group;
+          const int64_t at = (int64_t)(tile.first_token + tok) * p.q_sb + (int64_t)(head * p.group + g) * p.q_sh +
+                             (MAPS == 2 ? t * a.q_sm : 0) + c * 8;
+          x = __ldg(reinterpret_cast<const uint4*>((const __half*)p.q + at));
+        }
+        sts128(q0 + t * C::QTILE + (c / 8) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), x);
+      }
+      fence_proxy_async();
+      mbar_arrive(q_full);
+    }
+
+    const int limit = me < n_rows ? tc_limit(tile, first_row + me, p.group) : 0;
+    const int least = n_rows ? tc_limit(tile, first_row, p.group) : 0;  // the tile's row that sees the fewest
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = j0; j < end[t]; ++j) {
+      ok = mbar_wait(s_full + 8 * t, (uint32_t)(j - j0) & 1u, p.status, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const int bad = meta[j & (kTcMetaRing - 1)];
+      const bool masked = (j + 1) * kTcBlock > least || bad;
+      const int room = limit - j * kTcBlock;  // columns below this one are seen
+      const float* ks = SCALED ? scales + (j % C::SCALE_RING) * C::SCALE_FLOATS + (MAPS == 2 ? t * 128 : 0) : nullptr;
+      const float* vs = SCALED ? scales + (j % C::SCALE_RING) * C::SCALE_FLOATS + C::KT * 128 : nullptr;
+      // 32 scores at a time: K's scales and the mask
+      auto shape_scores = [&](float* x, int c0) {
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(ks + c0 + c);
+            x[c] *= f.x;
+            x[c + 1] *= f.y;
+            x[c + 2] *= f.z;
+            x[c + 3] *= f.w;
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (c0 + c >= room || ((bad >> ((c0 + c) / 16)) & 1)) x[c] = -INFINITY;
+        }
+      };
+      // The row's maximum; 16-bit pages keep the 128 scores in registers, 8-bit ones (more warps, fewer
+      // registers) read them from tensor memory again.
+      constexpr bool HOLD = !C::WIDEN;
+      float x[HOLD ? 128 : 32];
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if constexpr (HOLD) {
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) tc_ld32(s_at + c0, reinterpret_cast<uint32_t*>(x + c0));
+        tc_wait_ld();
+      }
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        float* y = HOLD ? x + c0 : x;
+        if constexpr (!HOLD) {
+          tc_ld32(s_at + c0, reinterpret_cast<uint32_t*>(y));
+          tc_wait_ld();
+        }
+        shape_scores(y, c0);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], y[c]);
+      }
+      const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+      if (j == j0) {
+        m = top;
+      } else if (__any_sync(kFull, top > m + kLag)) {
+        // O is that of the blocks before: this block's scores were issued behind their products
+        const float alpha = top == -INFINITY ? 1.f : fast_exp2(m - top);
+#pragma unroll 1
+        for (int c0 = 0; c0 < C::DV; c0 += 32) {
+          float o[32];
+          tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+          tc_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] *= alpha;
+          tc_st32(o_at + c0, reinterpret_cast<const uint32_t*>(o));
+        }
+        l *= alpha;
+        m = top;
+      }
+      const float from = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        float* y = HOLD ? x + c0 : x;
+        if constexpr (!HOLD) {
+          tc_ld32(s_at + c0, reinterpret_cast<uint32_t*>(y));
+          tc_wait_ld();
+          shape_scores(y, c0);
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          y[c] = fast_exp2(fmaf(y[c], p.scale_log2, -from));
+          sum[c & 3] += y[c];
+        }
+        uint32_t pk[16];
+#pragma unroll
+        for (int z = 0; z < C::NP; ++z) {
+          if constexpr (SCALED) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(vs + z * 128 + c0 + c);
+              pk[c / 2] = tc_pack<C::BF16>(y[c] * f.x, y[c + 1] * f.y);
+              pk[c / 2 + 1] = tc_pack<C::BF16>(y[c + 2] * f.z, y[c + 3] * f.w);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) pk[c / 2] = tc_pack<C::BF16>(y[c], y[c + 1]);
+          }
+          // columns below 16 (or 32) * (c0 / 32 + 1) hold scores that have been read
+          tc_st16(s_at + (C::NP == 1 ? c0 / 2 : c0 + 16 * z), pk);
+        }
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_full + 8 * t);
+    }
+
+    // ---- results ----------------------------------------------------------------------------------------
+    if (ok && end[t] > j0) ok = mbar_wait(o_done + 8 * t, 0, p.status, abort_flag);
+    tc_fence_after();
+    const bool any = end[t] > j0;  // else tensor memory holds nothing of this tile
+    const float inv = l > 0.f || l != l ? 1.f / (l * kBoost) : 0.f;
+    const bool live = me < n_rows;
+    const int pr = first_row + (live ? me : 0);
+    const int tok = pr / p.group, g = pr - tok * p.group;
+    const int64_t row = tile.first_token + tok;
+    const int hq = head * p.group + g;  // query head, or pair
+    if (tp.splits > 1) {
+      const int64_t at = (((int64_t)split * a.rows + row) * (p.hq / MAPS) + hq) * MAPS + (MAPS == 2 ? t : 0);
+#pragma unroll 1
+      for (int c0 = 0; c0 < C::DV; c0 += 32) {
+        float o[32];
+        if (any) {
+          tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+          tc_wait_ld();
+        }
+        if (live && ok) {
+          float4* dst = reinterpret_cast<float4*>(tp.part_o + at * (MAPS * D) + slice * C::DV + c0);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            dst[c / 4] = any && inv != 0.f ? make_float4(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      if (live && ok && slice == 0) tp.part_lse[at] = l > 0.f || l != l ? m + log2f(l) : -INFINITY;
+    } else if constexpr (MAPS == 1) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < C::DV; c0 += 32) {
+        float o[32];
+        if (any) {
+          tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+          tc_wait_ld();
+        }
+        if (live && ok) {
+          uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh + c0);
+          const bool some = any && inv != 0.f;
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {
+            uint4 y = make_uint4(0, 0, 0, 0);
+            if (some) {
+              y.x = tc_pack<C::BF16>(o[c] * inv, o[c + 1] * inv);
+              y.y = tc_pack<C::BF16>(o[c + 2] * inv, o[c + 3] * inv);
+              y.z = tc_pack<C::BF16>(o[c + 4] * inv, o[c + 5] * inv);
+              y.w = tc_pack<C::BF16>(o[c + 6] * inv, o[c + 7] * inv);
+            }
+            dst[c / 8] = y;
+          }
+        }
+      }
+    } else {
+      // The second map's rows reach the first map's threads through the ring (every tile in it has been
+      // read), a column of 128 rows at a time: neighbouring lanes, neighbouring words.
+      float* pass = reinterpret_cast<float*>(smem);
+      static_assert(C::NSLOT * C::SLOT >= 128 * 128 * 4, "room for one tile of f32");
+      const float lam = a.lambda(row, hq);
+      if (t == 1) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          float o[32];
+          if (any) {
+            tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+            tc_wait_ld();
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pass[(c0 + c) * 128 + me] = any && inv != 0.f ? o[c] * inv * lam : 0.f;
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      float square = 0.f;
+      if (t == 0) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          float o[32];
+          if (any) {
+            tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+            tc_wait_ld();
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float y = (any && inv != 0.f ? o[c] * inv : 0.f) - pass[(c0 + c) * 128 + me];
+            pass[(c0 + c) * 128 + me] = y;
+            square = fmaf(y, y, square);
+          }
+        }
+      }
+      if constexpr (C::SLICES == 2) {
+        if (t == 0) {  // this half's sum of squares to the other half's CTA
+          uint32_t peer;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(squares + me)), "r"(slice ^ 1));
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer), "f"(square) : "memory");
+        }
+      }
+      // the rest of the store waits for the cluster (below), with the same threads
+      if constexpr (C::SLICES == 1) {
+        if (t == 0 && live && ok) {
+          float factor = a.out_scale;
+          if (a.norm) factor *= rsqrtf(square * (1.f / (MAPS * D)) + a.eps);
+          uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh);
+#pragma unroll 4
+          for (int c = 0; c < 128; c += 8) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = pass[(c + e) * 128 + me] * factor * (a.weight ? __ldg(a.weight + c + e) : 1.f);
+            dst[c / 8] = make_uint4(tc_pack<C::BF16>(y[0], y[1]), tc_pack<C::BF16>(y[2], y[3]), tc_pack<C::BF16>(y[4], y[5]),
+                                    tc_pack<C::BF16>(y[6], y[7]));
+          }
+        }
+      } else {
+        squares[128 + me] = square;  // (t = 1 writes zeros first; see the order below)
+      }
+    }
+  }
+  // ---- the other half's sums of squares (head_dim 128, maps = 2) --------------------------------------------
+  if constexpr (C::SLICES == 2) {
+    if (tp.splits == 1) {
+      __syncthreads();
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (warp < 4) {
+        const int me = tid;
+        const bool live = me < tile.count && !*abort_flag;
+        if (live) {
+          const int pr = tile.row0 + me, tok = pr / p.group, hq = head * p.group + pr - tok * p.group;
+          const float* pass = reinterpret_cast<const float*>(smem);
+          const int64_t row = tile.first_token + tok;
+          float own = 0.f;
+          for (int c = 0; c < 128; ++c) own = fmaf(pass[c * 128 + me], pass[c * 128 + me], own);
+          float factor = a.out_scale;
+          if (a.norm) factor *= rsqrtf((own + squares[me]) * (1.f / (MAPS * D)) + a.eps);
+          uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh + slice * 128);
+#pragma unroll 4
+          for (int c = 0; c < 128; c += 8) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              y[e] = pass[(c + e) * 128 + me] * factor * (a.weight ? __ldg(a.weight + slice * 128 + c + e) : 1.f);
+            dst[c / 8] = make_uint4(tc_pack<C::BF16>(y[0], y[1]), tc_pack<C::BF16>(y[2], y[3]), tc_pack<C::BF16>(y[4], y[5]),
+                                    tc_pack<C::BF16>(y[6], y[7]));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+}  // namespace pd

@@ -21,6 +21,11 @@ PD_STREAM_LAUNCHER(stream_launch_bf16);
 PD_STREAM_LAUNCHER(stream_launch_e5m2);
 PD_STREAM_LAUNCHER(stream_launch_e5m2_scaled);
 PD_STREAM_LAUNCHER(stream_launch_i8);
+PD_STREAM_LAUNCHER(diff_launch_f16);
+PD_STREAM_LAUNCHER(diff_launch_bf16);
+PD_STREAM_LAUNCHER(diff_launch_e5m2);
+PD_STREAM_LAUNCHER(diff_launch_e5m2_scaled);
+PD_STREAM_LAUNCHER(diff_launch_i8);
 #undef PD_STREAM_LAUNCHER
 
 // ---------------------------------------------------------------------------------------------
@@ -43,16 +48,17 @@ struct Shape {
 // Workers (CTAs x workers per CTA) the cells' boundary table in shared memory is sized for.
 constexpr int kMaxWorkers = 1024;
 
-static Shape derive(const PdDecodeArgs* a) {
+static Shape derive(const PdDecodeArgs* a, int maps = 1) {
   Shape s;
   s.hb = head_block(a->num_kv_heads);
   // head_dim 256: a consumer thread holds 64 accumulator and 32 query registers per n-tile, and
   // at 16 bits a stage of 8 consumer warps' worth would be 128 KB; so at most four heads per
   // block and four consumer warps per CTA
   const bool wide = a->head_dim == 256;
-  if (wide && s.hb > 4) s.hb = 4;
+  const bool diff_wide = maps == 2 && diff_is_wide(a->head_dim, a->num_q_heads / a->num_kv_heads);
+  if ((wide || diff_wide) && s.hb > 4) s.hb = 4;
   s.nhb = a->num_kv_heads / s.hb;
-  s.wpc = wide ? 4 / s.hb : base_workers_per_cta(s.hb);
+  s.wpc = maps == 2 ? diff_workers_per_cta(s.hb, diff_wide) : wide ? 4 / s.hb : base_workers_per_cta(s.hb);
   s.splits = a->num_splits > 0 ? a->num_splits : 1;
   const long long nv = (long long)s.nhb * a->batch * s.splits;
   s.nvseq = nv > INT32_MAX ? INT32_MAX : (int)nv;
@@ -154,7 +160,7 @@ struct WorkspaceLayout {
   int slots;
 };
 
-static WorkspaceLayout workspace_layout(const PdDecodeArgs* a, const Shape& s, int sm_count) {
+static WorkspaceLayout workspace_layout(const PdDecodeArgs* a, const Shape& s, int sm_count, int maps = 1) {
   WorkspaceLayout w;
   const int group = a->num_q_heads / a->num_kv_heads;
   w.slots = sm_count * s.wpc + s.nvseq;
@@ -164,7 +170,7 @@ static WorkspaceLayout workspace_layout(const PdDecodeArgs* a, const Shape& s, i
   w.ticket_bytes = ((uint64_t)a->batch * a->num_kv_heads + (uint64_t)w.slots * s.hb) * 4;
   w.lse_off = round_up64(w.ticket_bytes, 256);
   w.o_off = w.lse_off + round_up64((uint64_t)w.slots * s.hb * group * 4, 256);
-  w.total = w.o_off + round_up64((uint64_t)w.slots * s.hb * group * a->head_dim * 4, 256);
+  w.total = w.o_off + round_up64((uint64_t)w.slots * s.hb * group * maps * a->head_dim * 4, 256);
   return w;
 }
 
@@ -250,9 +256,11 @@ static bool get_tensor_map(const MapKey& k, CUtensorMap* out) {
 static int launch_stream(const PdDecodeArgs* a, const Params& p, const Shape& s, const SmemPlan& sm,
                          const WorkspaceLayout& wl, char* scratch, const CUtensorMap& mk,
                          const CUtensorMap& mv, int sm_count, bool counters_zero = false,
-                         const PushTargets* push = nullptr) {
+                         const PushTargets* push = nullptr, const DiffTail* diff = nullptr) {
   StreamParams sp;
   sp.p = p;
+  if (diff) sp.diff = *diff;
+  else memset(&sp.diff, 0, sizeof(sp.diff));
   sp.p.num_splits = s.splits;
   sp.p.part_lse = (float*)(scratch + wl.lse_off);
   sp.p.part_o = (float*)(scratch + wl.o_off);
@@ -280,6 +288,14 @@ static int launch_stream(const PdDecodeArgs* a, const Params& p, const Shape& s,
   // zero, so a caller that vouches for a workspace it cleared once skips the memset node.
   if (!counters_zero && cudaMemsetAsync(sp.tickets, 0, wl.ticket_bytes, st) != cudaSuccess) return PD_ERR_CUDA;
   cudaError_t e;
+  if (diff) {
+    auto* launch = a->kv_dtype == PD_KV_F16    ? diff_launch_f16
+                   : a->kv_dtype == PD_KV_BF16 ? diff_launch_bf16
+                   : a->kv_dtype == PD_KV_I8   ? diff_launch_i8
+                   : s.scaled                  ? diff_launch_e5m2_scaled
+                                               : diff_launch_e5m2;
+    return launch(a->head_dim, s.hb, sp, mk, mv, sm_count, sm.total, st) == cudaSuccess ? PD_OK : PD_ERR_CUDA;
+  }
   switch (a->kv_dtype) {
     case PD_KV_F16: e = stream_launch_f16(a->head_dim, s.hb, sp, mk, mv, sm_count, sm.total, st); break;
     case PD_KV_BF16: e = stream_launch_bf16(a->head_dim, s.hb, sp, mk, mv, sm_count, sm.total, st); break;
@@ -309,6 +325,96 @@ int stream_run(const PdDecodeArgs* a, Params& p, int sm_count, const PushTargets
     return PD_ERR_CUDA;
   return launch_stream(a, p, s, sm, wl, (char*)a->workspace, mk, mv, sm_count,
                        (a->flags & PD_FLAG_COUNTERS_ZERO) != 0, push);
+}
+
+// ---------------------------------------------------------------------------------------------
+// differential decode
+// ---------------------------------------------------------------------------------------------
+// The cache side and the sizes of a differential decode as a decode request: two heads to a pair.
+static PdDecodeArgs as_decode(const PdPrefillArgs* a) {
+  PdDecodeArgs d;
+  memset(&d, 0, sizeof(d));
+  d.q = a->q;
+  d.out = a->out;
+  d.q_stride_b = a->q_stride_t;
+  d.q_stride_h = a->q_stride_h;
+  d.out_stride_b = a->out_stride_t;
+  d.out_stride_h = a->out_stride_h;
+  d.k_cache = a->k_cache;
+  d.v_cache = a->v_cache;
+  d.kv_stride_block = a->kv_stride_block;
+  d.kv_stride_token = a->kv_stride_token;
+  d.kv_stride_head = a->kv_stride_head;
+  d.k_scale = a->k_scale;
+  d.v_scale = a->v_scale;
+  d.scale_stride_block = a->scale_stride_block;
+  d.scale_stride_token = a->scale_stride_token;
+  d.block_table = a->block_table;
+  d.block_table_stride = a->block_table_stride;
+  d.seq_lens = a->seq_lens;
+  d.batch = a->batch;
+  d.num_q_heads = a->num_q_heads;
+  d.num_kv_heads = a->num_kv_heads;
+  d.head_dim = a->head_dim;
+  d.block_size = a->block_size;
+  d.num_blocks = a->num_blocks;
+  d.max_blocks_per_seq = a->max_blocks_per_seq;
+  d.kv_dtype = a->kv_dtype;
+  d.io_dtype = a->io_dtype;
+  d.sm_scale = a->sm_scale;
+  d.block_n = a->block_size;
+  d.sm_count = a->sm_count;
+  d.status = a->status;
+  d.workspace = a->workspace;
+  d.workspace_bytes = a->workspace_bytes;
+  d.stream = a->stream;
+  return d;
+}
+
+int diff_stream_supports(const PdPrefillArgs* a) {
+  if (a->maps != 2 || a->query_start) return PD_ERR_UNSUPPORTED;
+  if (a->head_dim != 64 && a->head_dim != 128) return PD_ERR_UNSUPPORTED;
+  const PdDecodeArgs d = as_decode(a);
+  const int why = stream_supports(&d);
+  if (why != PD_OK) return why;
+  if (a->q_stride_m % 2) return PD_ERR_UNSUPPORTED;
+  if (a->norm_weight && ((uintptr_t)a->norm_weight % 16)) return PD_ERR_UNSUPPORTED;
+  const Shape s = derive(&d, 2);
+  SmemPlan sm;
+  return plan_smem(s, sm) ? PD_OK : PD_ERR_UNSUPPORTED;
+}
+
+uint64_t diff_stream_workspace_bytes(const PdPrefillArgs* a, int sm_count) {
+  const PdDecodeArgs d = as_decode(a);
+  return workspace_layout(&d, derive(&d, 2), sm_count, 2).total;
+}
+
+int diff_stream_run(const PdPrefillArgs* a, int sm_count) {
+  const PdDecodeArgs d = as_decode(a);
+  const Shape s = derive(&d, 2);
+  SmemPlan sm;
+  if (!plan_smem(s, sm)) return PD_ERR_UNSUPPORTED;
+  if ((long long)sm_count * s.wpc > kMaxWorkers) return PD_ERR_UNSUPPORTED;
+  const WorkspaceLayout wl = workspace_layout(&d, s, sm_count, 2);
+  if (!a->workspace || a->workspace_bytes < wl.total) return PD_ERR_WORKSPACE;
+  Params p;
+  fill_params(&d, p);
+  DiffTail t;
+  t.lam = a->lam;
+  t.lam_sb = a->lam_stride_t;
+  t.lam_sh = a->lam_stride_h;
+  t.weight = a->norm_weight;
+  t.lam_value = a->lam_value;
+  t.eps = a->eps;
+  t.out_scale = a->out_scale;
+  t.norm = a->norm;
+  t.q_sm = a->q_stride_m;
+  // encoded for every call: nothing is kept by a tensor's address
+  CUtensorMap mk, mv;
+  if (!encode_tensor_map_in_place(map_key(&d, s, d.k_cache), &mk) ||
+      !encode_tensor_map_in_place(map_key(&d, s, d.v_cache), &mv))
+    return PD_ERR_CUDA;
+  return launch_stream(&d, p, s, sm, wl, (char*)a->workspace, mk, mv, sm_count, false, nullptr, &t);
 }
 
 // ---------------------------------------------------------------------------------------------

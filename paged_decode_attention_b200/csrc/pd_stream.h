@@ -22,6 +22,12 @@ struct PushTargets;
 // `push`, every finished unit is also stored into the exchange buffers it names.
 int stream_run(const PdDecodeArgs* a, Params& p, int sm_count, const PushTargets* push = nullptr);
 
+// The streaming kernel's differential form (maps = 2, one new token per request): the same three
+// for PdPrefillArgs without query_start.
+int diff_stream_supports(const PdPrefillArgs* a);
+uint64_t diff_stream_workspace_bytes(const PdPrefillArgs* a, int sm_count);
+int diff_stream_run(const PdPrefillArgs* a, int sm_count);
+
 // Defined in pd_api.cu: argument checks that need no device, the device-side parameter block,
 // and the SM count of the current device (or the caller's override).
 int validate(const PdDecodeArgs* a, bool need_output = true);

@@ -63,6 +63,15 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 // Workers per CTA: eight consumer warps' worth (at most four workers).
 __host__ __device__ constexpr int base_workers_per_cta(int hb) { return 8 / hb < 4 ? 8 / hb : 4; }
 
+// The differential form holds twice the accumulators a thread.  Up to eight query heads of a group and
+// head_dim 128, or any group at 64, fit the 168 registers a thread of nine or ten warps has; groups
+// of 9..16 at head_dim 128 (128 accumulators) spilled 500 to 2000 bytes there, so they run four
+// consumer warps per CTA, which leaves 255.
+__host__ __device__ constexpr bool diff_is_wide(int d, int group) { return d > 64 && group > 8; }
+__host__ __device__ constexpr int diff_workers_per_cta(int hb, bool wide) {
+  return wide ? 4 / hb : 8 / hb < 2 ? 8 / hb : 2;
+}
+
 template <int KV, int D, int HB, bool SCALED>
 struct StreamCfg {
   static constexpr int EB = is_16bit(KV) ? 2 : 1;
@@ -82,8 +91,25 @@ struct StreamCfg {
   static constexpr int MT = D / 16;                          // 16-row tiles of head_dim in O^T
 };
 
+// What the differential form (MAPS = 2) needs besides the decode parameters: the weight of the
+// second map for (request, pair), the optional RMS norm over the 2 * head_dim results of a pair,
+// and the element stride between the two query rows of a pair.  There Params::q_sh and o_sh are the
+// strides between pairs, and Params::hq, hkv and group count heads as always (two to a pair).
+struct DiffTail {
+  const float* lam;      // NULL: lam_value for every row
+  int64_t lam_sb, lam_sh;
+  const float* weight;   // [2 * head_dim] or NULL: ones
+  float lam_value, eps, out_scale;
+  int32_t norm;
+  int64_t q_sm;
+  __device__ __forceinline__ float lambda(int64_t row, int pair) const {
+    return lam ? __ldg(lam + row * lam_sb + pair * lam_sh) : lam_value;
+  }
+};
+
 struct StreamParams {
   Params p;
+  DiffTail diff;
   int32_t nvseq, nhb, splits, nstage, wpc;
   uint32_t bar_off, meta_off, misc_off, prefix_off, count_off, bound_off;
   // Query staging: qstage_warp_bytes > 0 when the query rows of one kv head's group are one dense
@@ -342,13 +368,16 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 // MASKED: the last tile holds fewer than 16 live tokens (`valid`); full tiles skip every mask.
 // NT = 2 takes two consecutive tiles of the same request (two stages) as one 32-token softmax
 // step: one running-maximum update, one rescale, and two independent score chains in flight.
-template <int KV, int D, int HB, bool SCALED, int NG, bool MASKED, int NT = 1>
+// MAPS = 2 (differential attention): the scores are those of one kv head as always, the values
+// are the rows of both heads of its pair side by side (`second` tells which of the two this warp
+// has), so O^T has 2 * D rows; 8-bit pages scale P by each V head's own scale, hence two P^T.
+template <int KV, int D, int HB, bool SCALED, int NG, bool MASKED, int NT = 1, int MAPS = 1>
 __device__ __forceinline__ void consume_tile(
     const uint32_t (&kbase)[NT], const uint32_t (&scales)[NT], const int hkv, const int valid,
     const float scale_log2, const int lane,
     const uint32_t (&qb)[StreamCfg<KV, D, HB, SCALED>::KSTEPS][NG][2], const float (&qstep)[NG][2],
-    float (&m)[NG][2], float (&l)[NG][2], float (&o)[StreamCfg<KV, D, HB, SCALED>::MT][NG][4],
-    float (&psum)[NG][4]) {
+    float (&m)[NG][2], float (&l)[NG][2], float (&o)[MAPS * StreamCfg<KV, D, HB, SCALED>::MT][NG][4],
+    float (&psum)[SCALED ? MAPS : 1][NG][4], const int second = 0) {
   using C = StreamCfg<KV, D, HB, SCALED>;
   constexpr unsigned kFull = 0xffffffffu;
   const int gq = lane >> 2, tq = lane & 3;
@@ -455,20 +484,32 @@ __device__ __forceinline__ void consume_tile(
   }
 
   // ---- scale, mask, online softmax; P^T into B-operand layout ---------------------------------
-  float f[NT][2], vs[NT][2];  // score factors and V scales (times 256) of tokens g and g + 8
+  constexpr int PV = SCALED ? MAPS : 1;  // different P^T operands: one for each V head's scales
+  float f[NT][2], vs[PV][NT][2];  // score factors and V scales (times 256) of tokens g and g + 8
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
     f[u][0] = f[u][1] = scale_log2;
-    vs[u][0] = vs[u][1] = 1.f;
     if constexpr (SCALED) {
       const uint32_t sa = scales[u] + gq * hkv * 2;
       f[u][0] *= lds_half(sa);
       f[u][1] *= lds_half(sa + 8 * hkv * 2);
-      vs[u][0] = lds_half(sa + 1024) * 256.f;
-      vs[u][1] = lds_half(sa + 1024 + 8 * hkv * 2) * 256.f;
+#pragma unroll
+      for (int z = 0; z < PV; ++z) {
+        const uint32_t va = sa + 1024 + (MAPS == 2 ? 2 * (z - second) : 0);
+        vs[z][u][0] = lds_half(va) * 256.f;
+        vs[z][u][1] = lds_half(va + 8 * hkv * 2) * 256.f;
+        if constexpr (MASKED) {  // scales behind the last token may be NaN: 0 * NaN would stay
+          if (u == NT - 1) {
+            if (gq >= valid) vs[z][u][0] = 0.f;
+            if (gq + 8 >= valid) vs[z][u][1] = 0.f;
+          }
+        }
+      }
+    } else {
+      vs[0][u][0] = vs[0][u][1] = 1.f;
     }
   }
-  uint32_t pb[NT][NG][2];
+  uint32_t pb[PV][NT][NG][2];
   float alpha[NG][2];
   bool moved = false;
 #pragma unroll
@@ -517,8 +558,13 @@ __device__ __forceinline__ void consume_tile(
       sum0 += p0 + p2;
       sum1 += p1 + p3;
       // (token g | g+8, heads 2t, 2t+1) -> (tokens 2t, 2t+1 | 2t+8, 2t+9, head g)
-      pb[u][ng][0] = movmatrix_trans(SCALED ? pack_io2<KV>(p0 * vs[u][0], p1 * vs[u][0]) : pack_io2<KV>(p0, p1));
-      pb[u][ng][1] = movmatrix_trans(SCALED ? pack_io2<KV>(p2 * vs[u][1], p3 * vs[u][1]) : pack_io2<KV>(p2, p3));
+#pragma unroll
+      for (int z = 0; z < PV; ++z) {
+        pb[z][u][ng][0] =
+            movmatrix_trans(SCALED ? pack_io2<KV>(p0 * vs[z][u][0], p1 * vs[z][u][0]) : pack_io2<KV>(p0, p1));
+        pb[z][u][ng][1] =
+            movmatrix_trans(SCALED ? pack_io2<KV>(p2 * vs[z][u][1], p3 * vs[z][u][1]) : pack_io2<KV>(p2, p3));
+      }
     }
     l[ng][0] = l[ng][0] * alpha[ng][0] + sum0;
     l[ng][1] = l[ng][1] * alpha[ng][1] + sum1;
@@ -526,7 +572,7 @@ __device__ __forceinline__ void consume_tile(
   // the running maxima settle after the first tiles; skip the rescale when nobody's moved
   if (__any_sync(kFull, moved)) {
 #pragma unroll
-    for (int mt = 0; mt < C::MT; ++mt) {
+    for (int mt = 0; mt < MAPS * C::MT; ++mt) {
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng) {
         o[mt][ng][0] *= alpha[ng][0];
@@ -537,11 +583,14 @@ __device__ __forceinline__ void consume_tile(
     }
     if constexpr (KV == PD_KV_I8) {
 #pragma unroll
-      for (int ng = 0; ng < NG; ++ng) {
-        psum[ng][0] *= alpha[ng][0];
-        psum[ng][1] *= alpha[ng][1];
-        psum[ng][2] *= alpha[ng][0];
-        psum[ng][3] *= alpha[ng][1];
+      for (int z = 0; z < PV; ++z) {
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) {
+          psum[z][ng][0] *= alpha[ng][0];
+          psum[z][ng][1] *= alpha[ng][1];
+          psum[z][ng][2] *= alpha[ng][0];
+          psum[z][ng][3] *= alpha[ng][1];
+        }
       }
     }
   }
@@ -556,8 +605,10 @@ __device__ __forceinline__ void consume_tile(
     keep_hi = (2 * tq + 8 < valid ? 0x0000ffffu : 0u) | (2 * tq + 9 < valid ? 0xffff0000u : 0u);
   }
 #pragma unroll
-  for (int u = 0; u < NT; ++u) {
-    const uint32_t vbase = kbase[u] + C::TILE_BYTES;
+  for (int uz = 0; uz < NT * MAPS; ++uz) {
+    const int u = uz / MAPS, z = uz % MAPS;  // tile, V head of the pair
+    const int pz = SCALED ? z : 0;
+    const uint32_t vbase = kbase[u] + C::TILE_BYTES + (MAPS == 2 ? (z - second) * (kTileTokens * C::PITCH) : 0);
     const bool mask_this = kMaskV && u == NT - 1;
     if constexpr (is_16bit(KV)) {
       // transposed 8x8 matrices (tokens 0-7, lo), (0-7, hi), (8-15, lo), (8-15, hi) of the 16
@@ -578,7 +629,7 @@ __device__ __forceinline__ void consume_tile(
           a[3] &= keep_hi;
         }
 #pragma unroll
-        for (int ng = 0; ng < NG; ++ng) mma_kv<KV>(o[mt][ng], a, pb[u][ng][0], pb[u][ng][1]);
+        for (int ng = 0; ng < NG; ++ng) mma_kv<KV>(o[z * C::MT + mt][ng], a, pb[pz][u][ng][0], pb[pz][u][ng][1]);
       }
     } else {
       // 8-bit V: from each of its four tokens the thread reads BPT = PITCH / 8 contiguous bytes
@@ -629,7 +680,7 @@ __device__ __forceinline__ void consume_tile(
               a[3] &= keep_hi;
             }
 #pragma unroll
-            for (int ng = 0; ng < NG; ++ng) mma_kv<KV>(o[mt][ng], a, pb[u][ng][0], pb[u][ng][1]);
+            for (int ng = 0; ng < NG; ++ng) mma_kv<KV>(o[z * C::MT + mt][ng], a, pb[pz][u][ng][0], pb[pz][u][ng][1]);
           }
         }
       }
@@ -642,9 +693,12 @@ __device__ __forceinline__ void consume_tile(
     // accumulator once, when the segment ends (no multiply-add per accumulator and tile).
     const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng) {
+    for (int z = 0; z < PV; ++z) {
 #pragma unroll
-      for (int u = 0; u < NT; ++u) mma_kv<KV>(psum[ng], ones, pb[u][ng][0], pb[u][ng][1]);
+      for (int ng = 0; ng < NG; ++ng) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) mma_kv<KV>(psum[z][ng], ones, pb[z][u][ng][0], pb[z][u][ng][1]);
+      }
     }
   }
 }
@@ -828,10 +882,119 @@ __device__ __forceinline__ void merge_unit(const Params& p, const int* prefix, c
   }
 }
 
+// The last step of a differential pair: both maps' partials are merged as in merge_unit (their
+// rows interleaved, so that lane groups q and q ^ 1 hold the two maps of one query row), then
+//   x = o1 - lambda * o2,   out = x * rsqrt(mean(x^2) + eps) * weight * out_scale
+// over the 2 * D results of the row.  The inputs are the n slots slot0, slot0 + stride, ...; the
+// pair's first kv head is `head0` in its block.  Everything stays in 32 bits up to the store.
+template <int KV, int D>
+__device__ __forceinline__ void merge_pair(const StreamParams& sp, int hg, int head0, int b, int pair, int lane,
+                                           int slot0, int n, int stride) {
+  constexpr int DV = 2 * D, J = DV / 16;
+  constexpr unsigned kFull = 0xffffffffu;
+  const Params& p = sp.p;
+  const int q = lane >> 2, c = lane & 3;
+  const int rows = 2 * p.group;
+  int rp = 2;
+  while (rp < rows && rp < 8) rp <<= 1;
+  const int phases = 8 / rp, phase = q / rp;
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    const int row = r0 + q % rp;
+    const bool live = row < rows;
+    const int g = live ? row >> 1 : 0;
+    const int64_t local = (int64_t)(head0 + (row & 1)) * p.group + g;
+    float m = -INFINITY, denom = 0.f;
+    float acc[J][4];
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    for (int i = phase; i < n; i += phases) {
+      const int64_t sr = ((int64_t)slot0 + (int64_t)i * stride) * hg + local;
+      const float lse = __ldcg(p.part_lse + sr);
+      const float4* op = reinterpret_cast<const float4*>(p.part_o + sr * DV) + c;
+      float4 x[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) x[j] = __ldcg(op + 4 * j);
+      if (lse > m) {
+        const float down = m > -INFINITY ? exp2f(m - lse) : 0.f;
+        denom *= down;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          acc[j][0] *= down;
+          acc[j][1] *= down;
+          acc[j][2] *= down;
+          acc[j][3] *= down;
+        }
+        m = lse;
+      }
+      const float wgt = lse > -INFINITY ? exp2f(lse - m) : 0.f;
+      denom += wgt;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        acc[j][0] = fmaf(wgt, x[j].x, acc[j][0]);
+        acc[j][1] = fmaf(wgt, x[j].y, acc[j][1]);
+        acc[j][2] = fmaf(wgt, x[j].z, acc[j][2]);
+        acc[j][3] = fmaf(wgt, x[j].w, acc[j][3]);
+      }
+    }
+    if (phases > 1) {
+      float mall = m;
+      for (int sh = 4 * rp; sh < 32; sh <<= 1) mall = fmaxf(mall, __shfl_xor_sync(kFull, mall, sh));
+      const float down = m > -INFINITY ? exp2f(m - mall) : 0.f;
+      denom *= down;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        acc[j][0] *= down;
+        acc[j][1] *= down;
+        acc[j][2] *= down;
+        acc[j][3] *= down;
+      }
+      for (int sh = 4 * rp; sh < 32; sh <<= 1) {
+        denom += __shfl_xor_sync(kFull, denom, sh);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] += __shfl_xor_sync(kFull, acc[j][e], sh);
+        }
+      }
+    }
+    // the even lane group of a pair of groups has the first map, its neighbour the second
+    const int head = pair * p.group + g;
+    const float inv = denom > 0.f ? 1.f / denom : 0.f;
+    const float lam = sp.diff.lambda(b, head);
+    float square = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mine = acc[j][e] * inv;
+        const float x = mine - lam * __shfl_xor_sync(kFull, mine, 4);
+        acc[j][e] = x;
+        square = fmaf(x, x, square);
+      }
+    }
+    square += __shfl_xor_sync(kFull, square, 1);
+    square += __shfl_xor_sync(kFull, square, 2);
+    if (!live || phase != 0 || (row & 1)) continue;
+    float factor = sp.diff.out_scale;
+    if (sp.diff.norm) factor *= rsqrtf(square * (1.f / DV) + sp.diff.eps);
+    __half* dst = (__half*)p.out + (int64_t)b * p.o_sb + (int64_t)head * p.o_sh;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int col = 16 * j + 4 * c;
+      float4 wv = make_float4(1.f, 1.f, 1.f, 1.f);
+      if (sp.diff.weight) wv = __ldg(reinterpret_cast<const float4*>(sp.diff.weight + col));
+      uint2 pk;
+      pk.x = pack_io2<KV>(acc[j][0] * factor * wv.x, acc[j][1] * factor * wv.y);
+      pk.y = pack_io2<KV>(acc[j][2] * factor * wv.z, acc[j][3] * factor * wv.w);
+      *reinterpret_cast<uint2*>(dst + col) = pk;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // the kernel
 // ---------------------------------------------------------------------------------------------
-template <int KV, int D, int HB, bool SCALED, int NG, int WPC>
+template <int KV, int D, int HB, bool SCALED, int NG, int WPC, int MAPS = 1>
 __global__ void __launch_bounds__(WPC * (HB + 1) * 32, 1)
 stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v) {
@@ -975,6 +1138,11 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     for (int u = tid; u < sp.nhb * p.batch; u += kThreads) {
       if (prefix[(u + 1) * sp.splits] != prefix[u * sp.splits]) continue;
       const int b = u % p.batch, hb = u / p.batch;
+      if constexpr (MAPS == 2) {
+        for (int h = hb * HB * p.group / 2; h < (hb + 1) * HB * p.group / 2; ++h)
+          for (int d = 0; d < 2 * D; ++d) ((uint16_t*)p.out)[(int64_t)b * p.o_sb + (int64_t)h * p.o_sh + d] = 0;
+        continue;
+      }
       for (int h = hb * HB * p.group; h < (hb + 1) * HB * p.group; ++h) {
         for (int d = 0; d < D; ++d) {
           if (p.out) ((uint16_t*)p.out)[(int64_t)b * p.o_sb + (int64_t)h * p.o_sh + d] = 0;  // +0 in f16 and bf16
@@ -1089,8 +1257,12 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     const int vend = prefix[v + 1];
     const int seg_end = g1 < vend ? g1 : vend;
     int j = g - prefix[v];
-    const bool whole = (j == 0) && (seg_end == vend) && (sp.splits == 1) && !pushing;
+    const bool whole = MAPS == 1 && (j == 0) && (seg_end == vend) && (sp.splits == 1) && !pushing;
     const int kvh = vi.hb * HB + role;
+    // first query row of this kv head's group and the stride between the rows; the heads of a
+    // pair alternate in the cache (MAPS = 2), their query rows are q_sm apart
+    const int64_t q_first = MAPS == 2 ? (int64_t)(kvh >> 1) * p.group * p.q_sh + (kvh & 1) * sp.diff.q_sm
+                                      : (int64_t)kvh * p.group * p.q_sh;
 
     // ---- query rows of this kv head's group as B fragments: thread (g, t) holds head g (+8 per
     // n-tile), head_dim pairs of its k slots; heads >= group are zero --------------------------
@@ -1141,7 +1313,7 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     if (qstage) {
       fill_fragments([&](int head, int col) { return lds32(qstage + (uint32_t)head * kQPitch + 2u * (uint32_t)col); });
     } else {
-      const __half* qrows = (const __half*)p.q + (int64_t)vi.b * p.q_sb + (int64_t)kvh * p.group * p.q_sh;
+      const __half* qrows = (const __half*)p.q + (int64_t)vi.b * p.q_sb + q_first;
       fill_fragments([&](int head, int col) {
         return __ldg(reinterpret_cast<const uint32_t*>(qrows + (int64_t)head * p.q_sh + col));
       });
@@ -1195,28 +1367,41 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     // stream has long pushed q out of L2).  One 128-byte line per lane.
     if (seg_end < g1 && v + 1 < nv) {
       const VseqInfo nx = vseq_info(sp, v + 1);
-      const int lines = (p.group * D * 2 + 127) / 128;
-      if (lane < lines) {
-        const char* nq = (const char*)p.q + 2 * ((int64_t)nx.b * p.q_sb +
-                                                 (int64_t)(nx.hb * HB + role) * p.group * p.q_sh);
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(nq + 128 * lane));
+      if constexpr (MAPS == 2) {  // the group's rows lie q_sh apart: one or two lines each
+        constexpr int kLines = D * 2 / 128;
+        const int nkvh = nx.hb * HB + role;
+        if (lane < p.group * kLines) {
+          const char* nq = (const char*)p.q + 2 * ((int64_t)nx.b * p.q_sb + (int64_t)(nkvh >> 1) * p.group * p.q_sh +
+                                                   (nkvh & 1) * sp.diff.q_sm + (int64_t)(lane / kLines) * p.q_sh);
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(nq + 128 * (lane % kLines)));
+        }
+      } else {
+        const int lines = (p.group * D * 2 + 127) / 128;
+        if (lane < lines) {
+          const char* nq = (const char*)p.q + 2 * ((int64_t)nx.b * p.q_sb +
+                                                   (int64_t)(nx.hb * HB + role) * p.group * p.q_sh);
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(nq + 128 * lane));
+        }
       }
     }
 
     float m[NG][2], l[NG][2];
-    float o[C::MT][NG][4];
+    float o[MAPS * C::MT][NG][4];
 #pragma unroll
     for (int ng = 0; ng < NG; ++ng) {
       m[ng][0] = m[ng][1] = -INFINITY;
       l[ng][0] = l[ng][1] = 0.f;
     }
 #pragma unroll
-    for (int mt = 0; mt < C::MT; ++mt)
+    for (int mt = 0; mt < MAPS * C::MT; ++mt)
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng) o[mt][ng][0] = o[mt][ng][1] = o[mt][ng][2] = o[mt][ng][3] = 0.f;
-    float psum[NG][4];  // int8 pages: running column sums of P^T (see consume_tile)
+    constexpr int PV = SCALED ? MAPS : 1;
+    float psum[PV][NG][4];  // int8 pages: running column sums of P^T (see consume_tile)
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng) psum[ng][0] = psum[ng][1] = psum[ng][2] = psum[ng][3] = 0.f;
+    for (int z = 0; z < PV; ++z)
+#pragma unroll
+      for (int ng = 0; ng < NG; ++ng) psum[z][ng][0] = psum[z][ng][1] = psum[z][ng][2] = psum[z][ng][3] = 0.f;
 
     // 8-bit tiles with a deep ring (five stages or more) are taken two at a time: one softmax
     // step per 32 tokens and two independent score chains per warp.  With fewer stages the
@@ -1247,11 +1432,11 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
             const uint32_t sc[2] = {sbase + 2 * C::TILE_BYTES + kvh * 2, sbase1 + 2 * C::TILE_BYTES + kvh * 2};
             const int remaining1 = remaining - kTileTokens;  // >= 1: the next tile is of this request
             if (remaining1 >= kTileTokens)
-              consume_tile<KV, D, HB, SCALED, NG, false, 2>(kb, sc, p.hkv, kTileTokens, p.scale_log2,
-                                                            lane, qb, qstep, m, l, o, psum);
+              consume_tile<KV, D, HB, SCALED, NG, false, 2, MAPS>(kb, sc, p.hkv, kTileTokens, p.scale_log2,
+                                                            lane, qb, qstep, m, l, o, psum, role & 1);
             else
-              consume_tile<KV, D, HB, SCALED, NG, true, 2>(kb, sc, p.hkv, remaining1, p.scale_log2,
-                                                           lane, qb, qstep, m, l, o, psum);
+              consume_tile<KV, D, HB, SCALED, NG, true, 2, MAPS>(kb, sc, p.hkv, remaining1, p.scale_log2,
+                                                           lane, qb, qstep, m, l, o, psum, role & 1);
             __syncwarp();
             if (lane == 0) {
               mbar_arrive(empty0 + 8 * st);
@@ -1269,11 +1454,11 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
         const uint32_t kb[1] = {sbase + role * (kTileTokens * C::PITCH)};
         const uint32_t sc[1] = {sbase + 2 * C::TILE_BYTES + kvh * 2};
         if (remaining >= kTileTokens)
-          consume_tile<KV, D, HB, SCALED, NG, false>(kb, sc, p.hkv, kTileTokens, p.scale_log2,
-                                                     lane, qb, qstep, m, l, o, psum);
+          consume_tile<KV, D, HB, SCALED, NG, false, 1, MAPS>(kb, sc, p.hkv, kTileTokens, p.scale_log2,
+                                                     lane, qb, qstep, m, l, o, psum, role & 1);
         else
-          consume_tile<KV, D, HB, SCALED, NG, true>(kb, sc, p.hkv, remaining, p.scale_log2,
-                                                    lane, qb, qstep, m, l, o, psum);
+          consume_tile<KV, D, HB, SCALED, NG, true, 1, MAPS>(kb, sc, p.hkv, remaining, p.scale_log2,
+                                                    lane, qb, qstep, m, l, o, psum, role & 1);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty0 + 8 * st);
@@ -1287,11 +1472,12 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     if constexpr (KV == PD_KV_I8) {
       // the surplus of the biased int8 values: 1152 times the column sums of P^T, rows alike
 #pragma unroll
-      for (int mt = 0; mt < C::MT; ++mt) {
+      for (int mt = 0; mt < MAPS * C::MT; ++mt) {
 #pragma unroll
         for (int ng = 0; ng < NG; ++ng) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[mt][ng][r] = fmaf(-1152.f, psum[ng][r], o[mt][ng][r]);
+          for (int r = 0; r < 4; ++r)
+            o[mt][ng][r] = fmaf(-1152.f, psum[SCALED ? mt / C::MT : 0][ng][r], o[mt][ng][r]);
         }
       }
     }
@@ -1318,13 +1504,13 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
           }
         } else {
           const int64_t slot_row = (int64_t)(w + v) * hg + role * p.group + head;
-          dst32 = p.part_o + slot_row * D;
+          dst32 = p.part_o + slot_row * (MAPS * D);
           if (gq == 0) p.part_lse[slot_row] = lse;
         }
         if constexpr (is_16bit(KV)) {
           // m-tile mt holds head_dim 16*mt + g (regs 0, 1) and 16*mt + g + 8 (regs 2, 3)
 #pragma unroll
-          for (int mt = 0; mt < C::MT; ++mt) {
+          for (int mt = 0; mt < MAPS * C::MT; ++mt) {
             const float x = o[mt][ng][e] * inv, y = o[mt][ng][2 + e] * inv;
             const int col = 16 * mt + gq;
             if (dst16) {
@@ -1341,7 +1527,7 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
           // word i of piece c came from m-tiles c*(PITCH/16) + 2*i and + 1 (rows g and g + 8)
           constexpr int WPT = C::PITCH / 32;
 #pragma unroll
-          for (int c = 0; c < C::NC; ++c) {
+          for (int c = 0; c < MAPS * C::NC; ++c) {
 #pragma unroll
             for (int i = 0; i < WPT; i += 2) {
               float x[8];
@@ -1375,14 +1561,18 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
       __threadfence();
       __syncwarp();
       const int v0 = (vi.hb * p.batch + vi.b) * sp.splits;
-      int* unit_ticket = sp.tickets + (int64_t)vi.b * p.hkv + kvh;
+      // Both maps of a differential pair report to one counter, the pair's first head's.
+      int* unit_ticket = sp.tickets + (int64_t)vi.b * p.hkv + (MAPS == 2 ? kvh & ~1 : kvh);
       // An unsplit request cut over more than kMergeRadix workers (one long request can span
       // every worker) is merged in two levels: chunks of kMergeRadix consecutive segments
       // first, each by the warp that completes the chunk, into the chunk's first slot; then
       // the chunk results by the warp that completes the unit.  The chunk merges of one
       // request run on different SMs at the same time.
       int wfirst = 0, nseg = 0;
-      if (sp.splits == 1) {
+      if (MAPS == 2 && dealt_whole) {
+        wfirst = w;  // the pair's two warps are in this worker; there is no boundary table
+        nseg = 1;
+      } else if (sp.splits == 1) {
         wfirst = cm.of(prefix[v0]);
         nseg = cm.of(prefix[v0 + 1] - 1) - wfirst + 1;
       }
@@ -1399,32 +1589,39 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
         }
         if (__shfl_sync(kFull, done, 0)) {
           __threadfence();
-          merge_unit<KV, D>(p, prefix, cm, v0, 1, hg, role, vi.b, kvh, lane, cslot, csize, 1, cslot);
+          merge_unit<KV, MAPS * D>(p, prefix, cm, v0, 1, hg, role, vi.b, kvh, lane, cslot, csize, 1, cslot);
           __threadfence();
           __syncwarp();
           int last = 0;
           if (lane == 0) {
-            last = atomicAdd(unit_ticket, 1) + 1 == nchunk;
+            last = atomicAdd(unit_ticket, 1) + 1 == MAPS * nchunk;
             if (last) *unit_ticket = 0;
           }
           if (__shfl_sync(kFull, last, 0)) {
             __threadfence();
-            merge_unit<KV, D>(p, prefix, cm, v0, 1, hg, role, vi.b, kvh, lane, wfirst + v0, nchunk,
-                              kMergeRadix, -1, pushing ? &sp.push : nullptr, *push_step);
+            if constexpr (MAPS == 2)
+              merge_pair<KV, D>(sp, hg, role & ~1, vi.b, kvh >> 1, lane, wfirst + v0, nchunk, kMergeRadix);
+            else
+              merge_unit<KV, D>(p, prefix, cm, v0, 1, hg, role, vi.b, kvh, lane, wfirst + v0, nchunk,
+                                kMergeRadix, -1, pushing ? &sp.push : nullptr, *push_step);
           }
         }
       } else {
         int last = 0;
         if (lane == 0) {
           int expected = 0;
-          for_each_segment(prefix, cm, v0, sp.splits, [&](int) { ++expected; });
+          if constexpr (MAPS == 2) expected = 2 * nseg;  // always unsplit
+          else for_each_segment(prefix, cm, v0, sp.splits, [&](int) { ++expected; });
           last = atomicAdd(unit_ticket, 1) + 1 == expected;
           if (last) *unit_ticket = 0;  // leave the counter as it was found
         }
         if (__shfl_sync(kFull, last, 0)) {
           __threadfence();
-          merge_unit<KV, D>(p, prefix, cm, v0, sp.splits, hg, role, vi.b, kvh, lane, 0, 0, 1, -1,
-                            pushing ? &sp.push : nullptr, *push_step);
+          if constexpr (MAPS == 2)
+            merge_pair<KV, D>(sp, hg, role & ~1, vi.b, kvh >> 1, lane, wfirst + v0, nseg, 1);
+          else
+            merge_unit<KV, D>(p, prefix, cm, v0, sp.splits, hg, role, vi.b, kvh, lane, 0, 0, 1, -1,
+                              pushing ? &sp.push : nullptr, *push_step);
         }
       }
     }

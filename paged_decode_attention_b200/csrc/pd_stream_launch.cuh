@@ -7,10 +7,10 @@
 
 namespace pd {
 
-template <int KV, int D, int HB, bool SCALED, int NG, int WPC>
+template <int KV, int D, int HB, bool SCALED, int NG, int WPC, int MAPS = 1>
 static inline cudaError_t launch_wpc(const StreamParams& sp, const CUtensorMap& mk, const CUtensorMap& mv,
                               int grid, uint32_t smem, cudaStream_t st) {
-  auto* kern = stream_decode_kernel<KV, D, HB, SCALED, NG, WPC>;
+  auto* kern = stream_decode_kernel<KV, D, HB, SCALED, NG, WPC, MAPS>;
   static bool configured[64] = {};  // per device: the opt-in shared-memory limit has been raised
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return cudaErrorInvalidDevice;
@@ -68,6 +68,37 @@ static inline cudaError_t launch_dtype(int head_dim, int hb, const StreamParams&
       else return cudaErrorInvalidValue;
     default: return cudaErrorInvalidValue;
   }
+}
+
+// The differential form: kv heads come in pairs, so a head block has two, four or eight; head_dim
+// 64 and 128 (a thread holds the accumulators of 2 * head_dim rows).
+template <int KV, int D, int HB, bool SCALED>
+static inline cudaError_t launch_diff_ng(const StreamParams& sp, const CUtensorMap& mk, const CUtensorMap& mv,
+                                         int grid, uint32_t smem, cudaStream_t st) {
+  if (sp.p.group <= 8)
+    return launch_wpc<KV, D, HB, SCALED, 1, diff_workers_per_cta(HB, false), 2>(sp, mk, mv, grid, smem, st);
+  constexpr bool wide = diff_is_wide(D, 16);
+  if constexpr (wide && HB > 4) return cudaErrorInvalidValue;
+  else return launch_wpc<KV, D, HB, SCALED, 2, diff_workers_per_cta(HB, wide), 2>(sp, mk, mv, grid, smem, st);
+}
+
+template <int KV, bool SCALED>
+static inline cudaError_t launch_diff(int head_dim, int hb, const StreamParams& sp, const CUtensorMap& mk,
+                                      const CUtensorMap& mv, int grid, uint32_t smem, cudaStream_t st) {
+  if (head_dim == 64) {
+    switch (hb) {
+      case 8: return launch_diff_ng<KV, 64, 8, SCALED>(sp, mk, mv, grid, smem, st);
+      case 4: return launch_diff_ng<KV, 64, 4, SCALED>(sp, mk, mv, grid, smem, st);
+      case 2: return launch_diff_ng<KV, 64, 2, SCALED>(sp, mk, mv, grid, smem, st);
+    }
+  } else if (head_dim == 128) {
+    switch (hb) {
+      case 8: return launch_diff_ng<KV, 128, 8, SCALED>(sp, mk, mv, grid, smem, st);
+      case 4: return launch_diff_ng<KV, 128, 4, SCALED>(sp, mk, mv, grid, smem, st);
+      case 2: return launch_diff_ng<KV, 128, 2, SCALED>(sp, mk, mv, grid, smem, st);
+    }
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace pd

@@ -1,0 +1,133 @@
+"""Block tables, slot maps, positions and lengths of one serving step, built on the GPU.
+
+``plan_step`` stands in front of ``cache_write`` and the attention entry points: from how many
+tokens each request has in the cache and how many it gets now, it takes the pages they lack from a
+free list, enters them into the block table, and returns where every new token goes.  Nothing is
+read back to the host, so a step (or a captured graph of steps) needs no synchronisation.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import typing
+
+import torch
+
+from . import _cabi
+from .decode import _call_on_device
+
+MAX_BATCH = 8192
+
+_PACK = _cabi.packer(_cabi.PdPlanArgs)
+
+
+class StepPlan(typing.NamedTuple):
+    """What ``plan_step`` returns; the names are those the other entry points use."""
+
+    slot_mapping: torch.Tensor  # [num_tokens] int64, -1: padding, or a token of a request not served
+    positions: torch.Tensor  # [num_tokens] int64, 0 for padding
+    query_start_loc: torch.Tensor  # [B + 1] int32
+    seq_lens: torch.Tensor  # [B] int32
+    num_free: torch.Tensor  # [1] int32
+
+
+def _vector(t: torch.Tensor, what: str, dtype: torch.dtype, size: int | None, device: torch.device) -> int:
+    if t.dtype != dtype or t.dim() != 1 or (size is not None and t.shape[0] != size):
+        raise ValueError(f"{what} must be a vector of {dtype}" + ("" if size is None else f" with {size} entries"))
+    if t.device != device:
+        raise ValueError(f"{what} must be on {device}")
+    if t.shape[0] > 1 and t.stride(0) != 1:
+        raise ValueError(f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def plan_step(block_table: torch.Tensor, context_lens: torch.Tensor, new_tokens: torch.Tensor,
+              free_blocks: torch.Tensor, num_free: torch.Tensor, *, block_size: int, num_tokens: int,
+              out: StepPlan | None = None, status: torch.Tensor | None = None) -> StepPlan:
+    """Plan one step of a batch.
+
+    ``block_table`` ``[B, max_blocks]``, ``context_lens`` ``[B]`` (tokens already cached) and
+    ``new_tokens`` ``[B]`` are int32; ``free_blocks`` holds the free block ids as a stack whose top
+    is entry ``num_free[0] - 1`` (both int32).  ``num_tokens`` is the length of the per-token
+    outputs: the sum of ``new_tokens``, or more for a padded batch.
+
+    Request b lacks ``ceil((c + n) / block_size) - ceil(c / block_size)`` pages; they are popped from
+    the stack in request order and written into its row of ``block_table`` (the only input that is
+    changed).  A request is served when its row has room for all its pages and the stack holds the
+    pages of all such requests up to and including it (or it needs none); one that is not served
+    keeps its length and row, its tokens get slot -1, and ``status`` (an int32 word) gets
+    ``DEV_NO_BLOCKS``.  Block ids are taken as they are; ``cache_write`` and the attention kernels
+    check them.
+
+    ``out`` receives the results in buffers of the caller, for captured graphs: ``out.seq_lens`` may
+    be ``context_lens`` and ``out.num_free`` may be ``num_free``, so a replayed step carries its state
+    on; otherwise nothing may overlap.  At most 8192 requests and fewer than 2**31 new tokens.
+    """
+    if not block_table.is_cuda:
+        raise _cabi.NativeLibraryError("plan_step runs on CUDA tensors only; there is no CPU path")
+    dev = block_table.device
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise ValueError("block_table must be int32 [batch, max_blocks]")
+    b, width = block_table.shape
+    if width > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table rows must be contiguous")
+    if b > 1 and block_table.stride(0) < width:
+        raise ValueError("block_table rows must not overlap")
+    num_tokens = int(num_tokens)
+    if num_tokens < 0 or int(block_size) <= 0:
+        raise ValueError("num_tokens must not be negative and block_size must be positive")
+    if b > MAX_BATCH:
+        raise ValueError(f"at most {MAX_BATCH} requests")
+    ctx = _vector(context_lens, "context_lens", torch.int32, b, dev)
+    new = _vector(new_tokens, "new_tokens", torch.int32, b, dev)
+    free = _vector(free_blocks, "free_blocks", torch.int32, None, dev)
+    nfree = _vector(num_free, "num_free", torch.int32, 1, dev)
+    if out is None:
+        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+        narrow = torch.empty(2 * b + 2, dtype=torch.int32, device=dev)
+        starts, lens, left = narrow.split((b + 1, b, 1))
+        out = StepPlan(slots, positions, starts, lens, left)
+        at = narrow.data_ptr()
+        ptrs = (slots.data_ptr(), positions.data_ptr(), at, at + 4 * (b + 1), at + 4 * (2 * b + 1))
+    else:
+        ptrs = (_vector(out.slot_mapping, "out.slot_mapping", torch.int64, num_tokens, dev),
+                _vector(out.positions, "out.positions", torch.int64, num_tokens, dev),
+                _vector(out.query_start_loc, "out.query_start_loc", torch.int32, b + 1, dev),
+                _vector(out.seq_lens, "out.seq_lens", torch.int32, b, dev),
+                _vector(out.num_free, "out.num_free", torch.int32, 1, dev))
+        _refuse_overlap(block_table, context_lens, new_tokens, free_blocks, num_free, out)
+    word = 0
+    if status is not None:
+        if status.dtype != torch.int32 or status.numel() < 1 or status.device != dev:
+            raise ValueError("status must be an int32 tensor on the same device")
+        word = status.data_ptr()
+    block = _PACK.pack(block_table.data_ptr(), max(block_table.stride(0), width), ctx, new, free, nfree, *ptrs, b, width,
+                       int(block_size), free_blocks.shape[0], num_tokens, word,
+                       torch.cuda.current_stream(dev).cuda_stream)
+    rc = _call_on_device(dev, _cabi.load().pd_plan_step, block)
+    if rc != 0:
+        _cabi.check(rc, "pd_plan_step")
+    return out
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    first = t.data_ptr()
+    last = first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else first
+    return first, last
+
+
+def _refuse_overlap(block_table, context_lens, new_tokens, free_blocks, num_free, out: StepPlan) -> None:
+    """No output shares memory with an input or another output, but for the two updates in place."""
+    inputs = [("block_table", block_table), ("context_lens", context_lens), ("new_tokens", new_tokens),
+              ("free_blocks", free_blocks), ("num_free", num_free)]
+    outputs = [(f"out.{n}", t) for n, t in zip(StepPlan._fields, out)]
+    for i, (name, t) in enumerate(outputs):
+        lo, hi = _span(t)
+        for other, u in inputs + outputs[:i]:
+            a, z = _span(u)
+            if lo < z and a < hi:
+                whole = (lo, hi) == (a, z)
+                if whole and (name, other) in (("out.seq_lens", "context_lens"), ("out.num_free", "num_free")):
+                    continue
+                raise ValueError(f"{name} overlaps {other}")

@@ -1,0 +1,212 @@
+"""Attention over the paged cache beyond one plain new token per request.
+
+* ``paged_prefill``: causal attention of many new tokens per request (prompts, chunks of prompts,
+  drafted tokens), a ragged batch in one call;
+* ``paged_diff_decode``: differential attention of one new token per request;
+* ``paged_diff_prefill``: differential attention of many new tokens per request.
+
+They read the cache that ``paged_decode`` reads, after ``cache_write`` has stored the new tokens.
+``kernel="auto"`` takes the kernels on the matrix units where they serve the request (head_dim 64
+and 128, pages of a multiple of 16 tokens up to 256, q of the cache's own 16-bit type or fp16 with
+8-bit pages, 16-byte aligned rows) and a general kernel on the CUDA cores everywhere else.  There
+is no CPU or PyTorch fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _cabi
+from .cache import PagedKVCache
+from .config import KV_CODE
+from .decode import _call_on_device
+
+_PACK = _cabi.packer(_cabi.PdPrefillArgs)
+_INDEX = {name: i for i, (name, _) in enumerate(_cabi.PdPrefillArgs._fields_)}
+_WORKSPACE, _WORKSPACE_BYTES = _INDEX["workspace"], _INDEX["workspace_bytes"]
+
+
+def build_prefill_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, query_start_loc: torch.Tensor | None, *,
+                       maps: int = 1, lam=None, norm: bool = False, norm_weight: torch.Tensor | None = None,
+                       eps: float = 1e-5, out_scale: float = 1.0, sm_scale: float | None = None, kernel: str = "auto",
+                       max_seq_len: int = 0, status: torch.Tensor | None = None, sm_count: int = 0,
+                       stream: int = 0) -> list:
+    """The checked values of a ``PdPrefillArgs`` block, in its field order, without scratch."""
+    k, v, bt, sl = cache.k_cache, cache.v_cache, cache.block_table, cache.seq_lens
+    dev = k.device
+    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+        raise ValueError("k_cache and v_cache must be alike [num_blocks, block_size, H_kv, D] with head_dim contiguous")
+    num_blocks, page, hkv, d = k.shape
+    hq = cache.shape.num_q_heads
+    if hkv != cache.shape.num_kv_heads or page != cache.block_size or d != cache.shape.head_dim:
+        raise ValueError("cache tensors disagree with cache.shape / cache.block_size")
+    if hq % maps or hkv % maps or hq % hkv:
+        raise ValueError(f"{hq} query heads and {hkv} kv heads do not form whole groups" + (" of pairs" if maps == 2 else ""))
+    if maps == 1:
+        if q.dim() != 3 or q.shape[1] != hq or q.shape[2] != d:
+            raise ValueError(f"q must be [rows, {hq}, {d}]")
+        map_stride = 0
+    else:
+        if q.dim() != 4 or q.shape[1] != hq // 2 or q.shape[2] != 2 or q.shape[3] != d:
+            raise ValueError(f"q must be [rows, {hq // 2}, 2, {d}]")
+        map_stride = q.stride(2)
+    if q.dtype not in _cabi.IO_CODE:
+        raise ValueError(f"q dtype {q.dtype} not supported (fp16 or bf16)")
+    if q.stride(-1) != 1:
+        raise ValueError("head_dim must be contiguous in q")
+    rows = q.shape[0]
+    if tuple(out.shape) != (rows, hq // maps, maps * d) or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be {q.dtype} [{rows}, {hq // maps}, {maps * d}] with the last dimension contiguous")
+    if bt.dtype != torch.int32 or sl.dtype != torch.int32 or bt.dim() != 2 or sl.dim() != 1:
+        raise ValueError("block_table [B, max_blocks] and seq_lens [B] must be int32")
+    if (bt.shape[1] > 1 and bt.stride(1) != 1) or not sl.is_contiguous():
+        raise ValueError("block_table rows and seq_lens must be contiguous")
+    b, width = bt.shape
+    if sl.shape[0] != b:
+        raise ValueError(f"seq_lens has {sl.shape[0]} entries for {b} block_table rows")
+    tensors = [q, out, v, bt, sl]
+    starts = 0
+    if query_start_loc is not None:
+        if query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1 or query_start_loc.shape[0] != b + 1 \
+                or not query_start_loc.is_contiguous():
+            raise ValueError(f"query_start_loc must be a contiguous int32 vector of {b + 1} entries")
+        starts = query_start_loc.data_ptr()
+        tensors.append(query_start_loc)
+    elif rows != b:
+        raise ValueError(f"q batch {rows} != block_table rows {b}")
+    ks, vs = cache.k_scale, cache.v_scale
+    scales = (0, 0, 0, 0)
+    if (ks is None) != (vs is None):
+        raise ValueError("k_scale and v_scale must both be given or both be None")
+    if ks is not None:
+        if ks.dtype != torch.float16 or vs.dtype != torch.float16 or tuple(ks.shape) != (num_blocks, page, hkv) \
+                or ks.shape != vs.shape or ks.stride() != vs.stride() or (hkv > 1 and ks.stride(2) != 1):
+            raise ValueError("scales must be fp16 [num_blocks, block_size, H_kv], alike, with the head index contiguous")
+        scales = (ks.data_ptr(), vs.data_ptr(), ks.stride(0), ks.stride(1))
+        tensors += (ks, vs)
+    lam_ptr, lam_t, lam_h, lam_value, weight = 0, 0, 0, 0.0, 0
+    if maps == 2:
+        if isinstance(lam, torch.Tensor):
+            if lam.dtype != torch.float32 or lam.dim() > 2:
+                raise ValueError("lam must be fp32: one value, [pairs] or [rows, pairs]")
+            lam = lam.expand(rows, hq // 2)  # raises when the shape does not broadcast
+            lam_ptr, lam_t, lam_h = lam.data_ptr(), lam.stride(0), lam.stride(1)
+            tensors.append(lam)
+        else:
+            lam_value = float(lam)
+        if norm_weight is not None:
+            if not norm:
+                raise ValueError("norm_weight without norm")
+            if norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (2 * d,) or not norm_weight.is_contiguous():
+                raise ValueError(f"norm_weight must be a contiguous fp32 vector of {2 * d} entries")
+            weight = norm_weight.data_ptr()
+            tensors.append(norm_weight)
+    word = 0
+    if status is not None:
+        if status.dtype != torch.int32 or status.numel() < 1:
+            raise ValueError("status must be an int32 tensor")
+        word = status.data_ptr()
+        tensors.append(status)
+    for t in tensors:
+        if t.device != dev:
+            raise ValueError(f"all tensors must be on {dev}, one is on {t.device}")
+    if kernel not in _cabi.KERNEL_CODE:
+        raise ValueError(f"kernel must be one of {sorted(_cabi.KERNEL_CODE)}")
+    return [q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), map_stride, out.stride(0), out.stride(1),
+            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), *scales,
+            bt.data_ptr(), max(bt.stride(0), width), sl.data_ptr(), starts,
+            rows, b, hq, hkv, d, page, num_blocks, width, KV_CODE[cache.kv_dtype], _cabi.IO_CODE[q.dtype],
+            cache.shape.softmax_scale if sm_scale is None else float(sm_scale), maps,
+            lam_ptr, lam_t, lam_h, lam_value, weight, float(eps), float(out_scale), int(bool(norm)),
+            _cabi.KERNEL_CODE[kernel], int(sm_count), int(max_seq_len), 0, 0, word, stream]
+
+
+def selected_prefill_kernel(values: list) -> str:
+    """Which kernel a block of ``build_prefill_args`` values runs on ("simple" or "stream")."""
+    rc = _cabi.load().pd_prefill_select_kernel(_PACK.pack(*values))
+    if rc < 0:
+        _cabi.check(rc, "pd_prefill_select_kernel")
+    return _cabi.KERNEL_NAME[rc]
+
+
+def _run(entry: str, q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor | None,
+         query_start_loc: torch.Tensor | None, maps: int, **kw) -> torch.Tensor:
+    if not q.is_cuda:
+        raise _cabi.NativeLibraryError(f"{entry} runs on CUDA tensors only; there is no CPU path")
+    dev = q.device
+    if out is None:
+        shape = (q.shape[0], q.shape[1], maps * q.shape[-1])
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    values = build_prefill_args(q, cache, out, query_start_loc, maps=maps,
+                                stream=torch.cuda.current_stream(dev).cuda_stream, **kw)
+    if q.shape[0] == 0 or cache.batch == 0:
+        return out
+    lib = _cabi.load()
+    need = ctypes.c_uint64(0)
+    block = _PACK.pack(*values)
+    rc = _call_on_device(dev, lib.pd_prefill_workspace_bytes, block, ctypes.byref(need))
+    if rc != 0:
+        _cabi.check(rc, "pd_prefill_workspace_bytes")
+    if need.value:
+        # Scratch of this call alone, from torch's allocator: ordered by the stream, and inside a
+        # capture a part of that graph, so no two graphs or streams share it.
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        values[_WORKSPACE], values[_WORKSPACE_BYTES] = ws.data_ptr(), need.value
+        block = _PACK.pack(*values)
+    rc = _call_on_device(dev, getattr(lib, entry), block)
+    if rc != 0:
+        _cabi.check(rc, entry)
+    return out
+
+
+def paged_prefill(q: torch.Tensor, cache: PagedKVCache, query_start_loc: torch.Tensor, out: torch.Tensor | None = None, *,
+                  sm_scale: float | None = None, kernel: str = "auto", max_seq_len: int = 0,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of many new tokens per request: q ``[T, Hq, D]`` -> ``[T, Hq, D]``.
+
+    Request b owns the rows ``query_start_loc[b] : query_start_loc[b + 1]`` (int32 ``[B + 1]``); they are
+    the last of its ``cache.seq_lens[b]`` cached tokens, and each attends to the keys up to its own
+    position.  Rows behind ``query_start_loc[B]`` are left as they were in ``out``; a request with more
+    rows than cached tokens has rows that attend to nothing, which are zero.  ``max_seq_len`` is an
+    optional host-side bound on ``seq_lens`` that refines how long contexts of few rows are split.
+    ``kernel`` and ``status`` are as for ``paged_decode``.
+    """
+    return _run("pd_prefill", q, cache, out, query_start_loc, 1, sm_scale=sm_scale, kernel=kernel,
+                max_seq_len=max_seq_len, status=status)
+
+
+def paged_diff_decode(q: torch.Tensor, cache: PagedKVCache, lam, out: torch.Tensor | None = None, *, norm: bool = True,
+                      norm_weight: torch.Tensor | None = None, eps: float = 1e-5, out_scale: float = 1.0,
+                      sm_scale: float | None = None, kernel: str = "auto",
+                      status: torch.Tensor | None = None) -> torch.Tensor:
+    """Differential attention of one new token per request: q ``[B, H, 2, D]`` -> ``[B, H, 2 * D]``.
+
+    The cache has two kv heads per kv pair: heads 2j and 2j + 1 are the keys K1 and K2 of pair j, and
+    their value rows side by side are its value V, ``2 * D`` wide.  ``cache.shape`` counts heads (``2 * H``
+    query heads).  With s = ``sm_scale`` (``D ** -0.5``) and ``lam`` a float or an fp32 tensor that
+    broadcasts to ``[B, H]``::
+
+        x   = softmax(q[:, :, 0] K1^T s) V - lam * softmax(q[:, :, 1] K2^T s) V
+        out = x * rsqrt(mean(x ** 2) + eps) * norm_weight * out_scale
+
+    ``norm=False`` leaves the norm out, ``norm_weight=None`` (fp32 ``[2 * D]``) its weight; a model's
+    constant factor behind the norm, one minus its initial lambda, is ``out_scale``.  A request of
+    length zero gives zeros.
+    """
+    return _run("pd_diff_decode", q, cache, out, None, 2, lam=lam, norm=norm, norm_weight=norm_weight, eps=eps,
+                out_scale=out_scale, sm_scale=sm_scale, kernel=kernel, status=status)
+
+
+def paged_diff_prefill(q: torch.Tensor, cache: PagedKVCache, query_start_loc: torch.Tensor, lam,
+                       out: torch.Tensor | None = None, *, norm: bool = True, norm_weight: torch.Tensor | None = None,
+                       eps: float = 1e-5, out_scale: float = 1.0, sm_scale: float | None = None, kernel: str = "auto",
+                       max_seq_len: int = 0, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Differential attention of many new tokens per request: q ``[T, H, 2, D]`` -> ``[T, H, 2 * D]``.
+
+    Rows and lengths as in ``paged_prefill``, the rest as in ``paged_diff_decode`` (``lam`` broadcasts to
+    ``[T, H]``).
+    """
+    return _run("pd_prefill", q, cache, out, query_start_loc, 2, lam=lam, norm=norm, norm_weight=norm_weight, eps=eps,
+                out_scale=out_scale, sm_scale=sm_scale, kernel=kernel, max_seq_len=max_seq_len, status=status)
