@@ -19,7 +19,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libpaged_decode_b200.so"
 SOURCES = ("pd_api.cu", "pd_stream.cu", "pd_stream_f16.cu", "pd_stream_bf16.cu", "pd_stream_e5m2.cu",
            "pd_stream_e5m2_scaled.cu", "pd_stream_i8.cu", "pd_diff_f16.cu", "pd_diff_bf16.cu", "pd_diff_e5m2.cu",
-           "pd_diff_e5m2_scaled.cu", "pd_diff_i8.cu", "pd_plan.cu", "pd_prefill.cu", "pd_prefill_tc.cu")
+           "pd_diff_e5m2_scaled.cu", "pd_diff_i8.cu", "pd_plan.cu", "pd_prefill.cu", "pd_prefill_tc.cu",
+           "pd_prefill_f16.cu", "pd_prefill_bf16.cu", "pd_prefill_e5m2.cu", "pd_prefill_e5m2_scaled.cu", "pd_prefill_i8.cu")
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -55,7 +55,7 @@ struct TcCfg {
   static constexpr int QTILE = 128 * D * 2;
   static constexpr int SLOT = 128 * (D > DV ? D : DV) * 2;
   static constexpr int SCALE_FLOATS = SCALED ? (KT + VH) * 128 : 0;  // of one block
-  static constexpr int SCALE_RING = 4;
+  static constexpr int SCALE_RING = 8;                     // more blocks than the ring of tiles can be ahead of the softmax
   static constexpr int FIXED = 1024 + 2 * QTILE + SCALE_RING * SCALE_FLOATS * 4 + 2048;
   static constexpr int FIT = (kTcSmem - FIXED) / SLOT;
   static constexpr int NSLOT = FIT > 8 ? 8 : FIT;
@@ -97,23 +97,25 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0)
       : "memory");
 }
-#define PD_R8(x, i) "=r"((x)[i]), "=r"((x)[i + 1]), "=r"((x)[i + 2]), "=r"((x)[i + 3]), "=r"((x)[i + 4]), \
-                    "=r"((x)[i + 5]), "=r"((x)[i + 6]), "=r"((x)[i + 7])
 #define PD_I8(x, i) "r"((x)[i]), "r"((x)[i + 1]), "r"((x)[i + 2]), "r"((x)[i + 3]), "r"((x)[i + 4]), \
                     "r"((x)[i + 5]), "r"((x)[i + 6]), "r"((x)[i + 7])
+#define PD_F8(x, i) "=f"((x)[i]), "=f"((x)[i + 1]), "=f"((x)[i + 2]), "=f"((x)[i + 3]), "=f"((x)[i + 4]), \
+                    "=f"((x)[i + 5]), "=f"((x)[i + 6]), "=f"((x)[i + 7])
+#define PD_G8(x, i) "f"((x)[i]), "f"((x)[i + 1]), "f"((x)[i + 2]), "f"((x)[i + 3]), "f"((x)[i + 4]), \
+                    "f"((x)[i + 5]), "f"((x)[i + 6]), "f"((x)[i + 7])
 // 32 columns of the warp's 32 lanes: thread = lane, register = column
-__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t* x) {
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float* x) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : PD_R8(x, 0), PD_R8(x, 8), PD_R8(x, 16), PD_R8(x, 24)
+      : PD_F8(x, 0), PD_F8(x, 8), PD_F8(x, 16), PD_F8(x, 24)
       : "r"(addr));
 }
-__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* x) {
+__device__ __forceinline__ void tc_st32(uint32_t addr, const float* x) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(addr), PD_I8(x, 0), PD_I8(x, 8), PD_I8(x, 16), PD_I8(x, 24)
+      ::"r"(addr), PD_G8(x, 0), PD_G8(x, 8), PD_G8(x, 16), PD_G8(x, 24)
       : "memory");
 }
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* x) {
@@ -257,6 +259,9 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   }
   __syncthreads();
   if (!*have_tile) return;  // the whole cluster has the same tile: nobody waits for this CTA
+  // the peer runs before anything is written to its shared memory
+  if (C::SLICES == 2 && tp.splits == 1)
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((const void*)tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -396,6 +401,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         const int st = unit % C::NSLOT;
         const uint32_t dst = ring0 + st * C::SLOT;
         const int pieces = (k < 0 ? C::DV : D) / 16;  // of one row; a warp-wide load covers whole rows
+        if (k == 0 && me == 0) meta[(j + kTcMetaRing / 2) & (kTcMetaRing - 1)] = 0;  // read long ago, written far ahead
         uint4 x[kMaxChunk];
 #pragma unroll
         for (int i = 0; i < kMaxChunk; ++i) {
@@ -416,22 +422,20 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             }
           }
         }
-        // the block's scales: one token a thread
-        float sc[SCALED ? C::VH : 1] = {};
+        // the block's scales, K's and V's, with its first K tile: the softmax needs them ahead of V itself
+        float sc[SCALED ? C::KT + C::VH : 1] = {};
         if constexpr (SCALED) {
           const int token = j * kTcBlock + me;
-          if (token < kv_end) {
+          if (k == 0 && token < kv_end) {
             const int page = token / p.page;
             const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
             if ((unsigned)id < (unsigned)p.num_blocks) {
-              if (k >= 0) {
-                sc[0] = __half2float(__ldg(p.k_scale + scale_offset(p, id, token - page * p.page, head * MAPS + k)));
-              } else {
+              const int64_t at = scale_offset(p, id, token - page * p.page, head * MAPS);
 #pragma unroll
-                for (int z = 0; z < C::VH; ++z)
-                  sc[z] = kBoost * __half2float(__ldg(p.v_scale + scale_offset(p, id, token - page * p.page,
-                                                                               head * MAPS + (MAPS == 2 ? slice * C::DV / D + z : 0))));
-              }
+              for (int z = 0; z < C::KT; ++z) sc[z] = __half2float(__ldg(p.k_scale + at + z));
+#pragma unroll
+              for (int z = 0; z < C::VH; ++z)
+                sc[C::KT + z] = kBoost * __half2float(__ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0)));
             }
           }
         }
@@ -450,9 +454,6 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             h[2 * e] = cvt_pair<KV>(y, false);
             h[2 * e + 1] = cvt_pair<KV>(y, true);
           }
-          if constexpr (KV == PD_KV_E5M2) {
-            // cvt_pair places bytes (0, 1) and (2, 3) above zero bytes, in order
-          }
           const uint32_t row = dst + (c / 4) * (128 * 128) + r * 128;
           const int ch = (2 * c) & 7;
           // neighbours that share banks store their two halves in opposite order
@@ -465,11 +466,10 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           }
         }
         if constexpr (SCALED) {
-          float* at = scales + (j % C::SCALE_RING) * C::SCALE_FLOATS;
-          if (k >= 0) at[k * 128 + me] = sc[0];
-          else {
+          if (k == 0) {
 #pragma unroll
-            for (int z = 0; z < C::VH; ++z) at[(C::KT + z) * 128 + me] = sc[z];
+            for (int z = 0; z < C::KT + C::VH; ++z)
+              scales[(j % C::SCALE_RING) * C::SCALE_FLOATS + z * 128 + me] = sc[z];
           }
         }
         fence_proxy_async();
@@ -634,14 +634,14 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if constexpr (HOLD) {
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) tc_ld32(s_at + c0, reinterpret_cast<uint32_t*>(x + c0));
+        for (int c0 = 0; c0 < 128; c0 += 32) tc_ld32(s_at + c0, x + c0);
         tc_wait_ld();
       }
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 32) {
         float* y = HOLD ? x + c0 : x;
         if constexpr (!HOLD) {
-          tc_ld32(s_at + c0, reinterpret_cast<uint32_t*>(y));
+          tc_ld32(s_at + c0, y);
           tc_wait_ld();
         }
         shape_scores(y, c0);
@@ -657,11 +657,11 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
 #pragma unroll 1
         for (int c0 = 0; c0 < C::DV; c0 += 32) {
           float o[32];
-          tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+          tc_ld32(o_at + c0, o);
           tc_wait_ld();
 #pragma unroll
           for (int c = 0; c < 32; ++c) o[c] *= alpha;
-          tc_st32(o_at + c0, reinterpret_cast<const uint32_t*>(o));
+          tc_st32(o_at + c0, o);
         }
         l *= alpha;
         m = top;
@@ -672,7 +672,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       for (int c0 = 0; c0 < 128; c0 += 32) {
         float* y = HOLD ? x + c0 : x;
         if constexpr (!HOLD) {
-          tc_ld32(s_at + c0, reinterpret_cast<uint32_t*>(y));
+          tc_ld32(s_at + c0, y);
           tc_wait_ld();
           shape_scores(y, c0);
         }
@@ -721,7 +721,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       for (int c0 = 0; c0 < C::DV; c0 += 32) {
         float o[32];
         if (any) {
-          tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+          tc_ld32(o_at + c0, o);
           tc_wait_ld();
         }
         if (live && ok) {
@@ -738,7 +738,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       for (int c0 = 0; c0 < C::DV; c0 += 32) {
         float o[32];
         if (any) {
-          tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+          tc_ld32(o_at + c0, o);
           tc_wait_ld();
         }
         if (live && ok) {
@@ -768,7 +768,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         for (int c0 = 0; c0 < 128; c0 += 32) {
           float o[32];
           if (any) {
-            tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+            tc_ld32(o_at + c0, o);
             tc_wait_ld();
           }
 #pragma unroll
@@ -782,7 +782,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         for (int c0 = 0; c0 < 128; c0 += 32) {
           float o[32];
           if (any) {
-            tc_ld32(o_at + c0, reinterpret_cast<uint32_t*>(o));
+            tc_ld32(o_at + c0, o);
             tc_wait_ld();
           }
 #pragma unroll
@@ -800,7 +800,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer), "f"(square) : "memory");
         }
       }
-      // the rest of the store waits for the cluster (below), with the same threads
+      // with two slices the store waits for the cluster (below)
       if constexpr (C::SLICES == 1) {
         if (t == 0 && live && ok) {
           float factor = a.out_scale;
@@ -815,8 +815,6 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
                                     tc_pack<C::BF16>(y[6], y[7]));
           }
         }
-      } else {
-        squares[128 + me] = square;  // (t = 1 writes zeros first; see the order below)
       }
     }
   }

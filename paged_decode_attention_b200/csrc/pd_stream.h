@@ -2,6 +2,8 @@
 // (pd_stream.cu).
 #pragma once
 
+#include <cuda.h>
+
 #include "pd_common.cuh"
 
 namespace pd {
@@ -27,6 +29,10 @@ int stream_run(const PdDecodeArgs* a, Params& p, int sm_count, const PushTargets
 int diff_stream_supports(const PdPrefillArgs* a);
 uint64_t diff_stream_workspace_bytes(const PdPrefillArgs* a, int sm_count);
 int diff_stream_run(const PdPrefillArgs* a, int sm_count);
+
+// Tensor map of one 16-bit cache tensor with boxes of 64 elements, `box_tokens` tokens and one head, in the
+// 128-byte swizzle.
+bool encode_page_box(const PdPrefillArgs* a, const void* cache, int box_tokens, CUtensorMap* out);
 
 // Defined in pd_api.cu: argument checks that need no device, the device-side parameter block,
 // and the SM count of the current device (or the caller's override).

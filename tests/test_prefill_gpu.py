@@ -118,7 +118,7 @@ def test_diff_decode_bad_blocks_are_left_out_and_flagged():
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (7, 1), (4, 2), (8, 1), (3, 3)])
 def test_prefill_heads_and_types(maps, kv, dim, heads, kv_heads):
-    both(ref.make([1, 17, 200, 130, 300], [1, 17, 200, 3, 129], heads=heads, kv_heads=kv_heads, dim=dim, kv=kv, maps=maps))
+    both(ref.make([1, 17, 200, 130, 300], [1, 17, 200, 3, 129], heads=heads, kv_heads=kv_heads, dim=dim, kv=kv, maps=maps), "stream")
 
 
 @pytest.mark.parametrize("maps", [1, 2])
@@ -128,14 +128,14 @@ def test_prefill_heads_and_types(maps, kv, dim, heads, kv_heads):
     ([300, 0, 300], [300, 0, 1]), ([3, 10], [7, 20]), ([0], [4])])
 def test_prefill_lengths(maps, lens, new):
     """Among them: no rows, no keys, more rows than keys (the first attend to nothing)."""
-    both(ref.make(lens, new, heads=4, kv_heads=2, dim=128, kv="bf16", maps=maps, seed=sum(lens)))
+    both(ref.make(lens, new, heads=4, kv_heads=2, dim=128, kv="bf16", maps=maps, seed=sum(lens)), "stream")
 
 
 @pytest.mark.parametrize("page", [16, 32, 48, 64, 128, 256])
 @pytest.mark.parametrize("kv", ["fp16", "fp8_e5m2"])
 def test_prefill_pages(page, kv):
     both(ref.make([1, page - 1, page, page + 1, 3 * page + 5], [1, page - 1, 3, page + 1, 2 * page], heads=4, kv_heads=2,
-                  page=page, kv=kv))
+                  page=page, kv=kv), "stream")
 
 
 @pytest.mark.parametrize("maps", [1, 2])
@@ -148,7 +148,7 @@ def test_prefill_on_the_general_kernel(maps, dim, page, kv, io):
 @pytest.mark.parametrize("how", [dict(norm=False), dict(weight=False), dict(lam="float"), dict(lam="rows"), dict(interleaved=True)])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_diff_prefill_options(how, dim):
-    both(ref.make([90, 200, 61], [90, 5, 40], heads=4, kv_heads=2, dim=dim, maps=2, seed=8, **how))
+    both(ref.make([90, 200, 61], [90, 5, 40], heads=4, kv_heads=2, dim=dim, maps=2, seed=8, **how), "stream")
 
 
 @pytest.mark.parametrize("maps", [1, 2])
