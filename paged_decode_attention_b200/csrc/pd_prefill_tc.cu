@@ -1,5 +1,5 @@
 // Host side of the prefill kernel on the matrix units (pd_prefill_tc.cuh): which requests it serves, how
-// they are split, tensor maps, launches, and the kernel that joins the splits.
+// they are split, launches, and the kernel that joins the splits.
 #include <cstring>
 
 #include "pd_prefill_tc.cuh"
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(128) tc_join_kernel(const TcParams tp, const i
 constexpr int kTcMaxSplits = 64;
 
 struct TcPlan {
-  int tiles, heads, splits, box_tokens;
+  int tiles, heads, splits;
   int64_t grid;
   uint64_t lse_off, bytes;
 };
@@ -110,8 +110,6 @@ static TcPlan tc_plan(const PdPrefillArgs* a, int sm_count) {
   const int group = a->num_q_heads / a->num_kv_heads;
   t.tiles = (int)((int64_t)a->num_rows * group / s.rows + a->batch);
   t.heads = a->num_kv_heads / a->maps;
-  t.box_tokens = 16;  // the largest power of two up to a block that divides the page
-  while (t.box_tokens < 128 && a->block_size % (2 * t.box_tokens) == 0) t.box_tokens *= 2;
   // Split the keys while the tiles do not fill the machine; a split keeps at least four blocks of the longest
   // context there can be.
   int64_t bound = (int64_t)a->max_blocks_per_seq * a->block_size;
@@ -136,7 +134,6 @@ int tc_supports(const PdPrefillArgs* a) {
   if (!a->query_start) return PD_ERR_UNSUPPORTED;
   if (a->head_dim != 64 && a->head_dim != 128) return PD_ERR_UNSUPPORTED;
   if ((a->kv_dtype == PD_KV_BF16) != (a->io_dtype == PD_IO_BF16)) return PD_ERR_UNSUPPORTED;
-  if (a->block_size % 16 != 0) return PD_ERR_UNSUPPORTED;
   if (!(a->sm_scale > 0.f) || a->sm_scale > 1e30f) return PD_ERR_UNSUPPORTED;  // the maximum is taken ahead of the factor
   const int group = a->num_q_heads / a->num_kv_heads;
   if (group > 128) return PD_ERR_UNSUPPORTED;
@@ -145,7 +142,7 @@ int tc_supports(const PdPrefillArgs* a) {
   const int64_t eb = a->kv_dtype <= PD_KV_BF16 ? 2 : 1;
   const int64_t strides[3] = {a->kv_stride_block, a->kv_stride_token, a->kv_stride_head};
   for (int64_t s : strides)
-    if (s < 0 || s * eb >= (1ll << 40)) return PD_ERR_UNSUPPORTED;
+    if (s < 0 || s * eb >= (1ll << 40)) return PD_ERR_UNSUPPORTED;  // limits of the tensor maps
   if ((int64_t)a->num_rows * group / 128 + a->batch > (1 << 30)) return PD_ERR_UNSUPPORTED;
   const TcShape s = tc_shape(a->head_dim, a->maps);
   const int64_t grid = ((int64_t)a->num_rows * group / s.rows + a->batch) * (a->num_kv_heads / a->maps) * s.slices;
@@ -162,14 +159,15 @@ int tc_run(const PdPrefillArgs* a, const PrefillParams& r, int sm_count) {
   tp.tiles = t.tiles;
   tp.heads = t.heads;
   tp.splits = t.splits;
-  tp.box_tokens = t.box_tokens;
   tp.part_o = t.bytes ? (float*)a->workspace : nullptr;
   tp.part_lse = t.bytes ? (float*)((char*)a->workspace + t.lse_off) : nullptr;
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
-  if (a->kv_dtype <= PD_KV_BF16) {  // encoded for every call: nothing is kept by a tensor's address
-    if (!encode_page_box(a, a->k_cache, t.box_tokens, &mk) || !encode_page_box(a, a->v_cache, t.box_tokens, &mv))
+  tp.box_tokens = 16;  // the largest power of two up to a block that divides the page
+  while (tp.box_tokens < kTcBlock && a->block_size % (2 * tp.box_tokens) == 0) tp.box_tokens *= 2;
+  if (a->kv_dtype <= PD_KV_BF16 && a->block_size % 16 == 0) {  // encoded for every call: nothing is kept by an address
+    if (!encode_page_box(a, a->k_cache, tp.box_tokens, &mk) || !encode_page_box(a, a->v_cache, tp.box_tokens, &mv))
       return PD_ERR_CUDA;
   }
   const cudaStream_t st = (cudaStream_t)a->stream;

@@ -16,7 +16,14 @@
 // on its four warps, the matrix units work for the other.  A thread owns one row, so maximum and sum
 // need no exchange.  S and O stay in tensor memory (2 * (128 + DV) columns), P replaces S there as
 // 16-bit pairs and is read by the second product from tensor memory; shared memory holds Q and a
-// ring of K and V tiles that one warp fills by TMA, page by page, in the 128-byte swizzle.
+// ring of K and V tiles in the 128-byte swizzle.
+//
+// Three warps fill the ring.  With pages of a multiple of 64 tokens everything comes by TMA.  TMA runs a
+// 16-token box (2 KB) in about 150 cycles, though, and a block has 32 of those, more than its products
+// take; so with smaller pages V comes by TMA and K by 16-byte asynchronous copies of two other warps, side
+// by side (8192 tokens, pages of 16: all TMA 634 us, all copies 749 us).  Copies also serve pages that are
+// no multiple of 16, and leave out what lies behind the last key; V's rows there are cleared behind the
+// copy, because zero times the NaN that a page may hold would stay.
 //
 // The maximum that P refers to may lag behind the true one by kLag (2^3 or 2^8 at most): O is then not
 // rescaled for every small rise.  It cancels in O / l; l and O are 32-bit.
@@ -51,16 +58,18 @@ struct TcCfg {
   static constexpr int VH = DV / D > 1 ? DV / D : 1;       // V heads side by side in the slice
   static constexpr int NP = SCALED ? VH : 1;               // different P operands (one for each V head's scales)
   static constexpr int KT = MAPS;                          // K tiles of one block
+  static constexpr int KH = D / 64, VC = DV / 64;          // 64-column pieces of a K and of a V row
   static constexpr int ROWS = MAPS == 2 ? 128 : 256;       // packed rows of one CTA
   static constexpr int QTILE = 128 * D * 2;
   static constexpr int SLOT = 128 * (D > DV ? D : DV) * 2;
   static constexpr int SCALE_FLOATS = SCALED ? (KT + VH) * 128 : 0;  // of one block
   static constexpr int SCALE_RING = 8;                     // more blocks than the ring of tiles can be ahead of the softmax
-  static constexpr int FIXED = 1024 + 2 * QTILE + SCALE_RING * SCALE_FLOATS * 4 + 2048;
+  static constexpr int MISC = 1024 + (MAPS == 2 ? 2560 : 0);
+  static constexpr int FIXED = 1024 + 2 * QTILE + SCALE_RING * SCALE_FLOATS * 4 + MISC;
   static constexpr int FIT = (kTcSmem - FIXED) / SLOT;
   static constexpr int NSLOT = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = FIXED + NSLOT * SLOT;
-  static constexpr int WARPS = WIDEN ? 14 : 10;            // softmax 0-3 and 4-7, loader 8, matrix units 9, widening 10-13
+  static constexpr int WARPS = WIDEN ? 14 : 12;            // softmax 0-3 and 4-7, matrix units 9, loaders 8, 10, 11 (or widening 10-13)
   static constexpr int THREADS = WARPS * 32;
   static_assert(NSLOT >= 3 && SMEM <= kTcSmem, "shared memory");
 };
@@ -76,25 +85,36 @@ struct TcParams {
 // ---- tcgen05 wrappers ----------------------------------------------------------------------------
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The matrix units' warp runs its loops as one and lets a single lane (`mine`) issue: operands then
+// live in the warp's uniform registers.  (Issued from inside a one-lane branch, an instruction took about
+// 100 cycles, most of it moving operands there.)
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t mine) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(bar), "r"(mine)
+      : "memory");
 }
 // D (128 x N, f32, tensor memory) (+)= A (128 x 16) * B (16 x N); A and B by shared-memory descriptors
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t mine) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0), "r"(mine)
       : "memory");
 }
 // the same with A in tensor memory (16-bit pairs)
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t mine) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1 : 0), "r"(mine)
       : "memory");
 }
 #define PD_I8(x, i) "r"((x)[i]), "r"((x)[i + 1]), "r"((x)[i + 2]), "r"((x)[i + 3]), "r"((x)[i + 4]), \
@@ -125,17 +145,42 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* x) {
       : "memory");
 }
 
-// Shared-memory operand descriptor in the 128-byte swizzle: 8-row groups 1024 bytes apart.  K-major
+// Where row r, piece c (64 columns, 128 bytes) of a Q, K or V tile lies: one plane of 128 rows a piece.
+__device__ __forceinline__ uint32_t tc_row(int r, int c) { return (uint32_t)(c * (128 * 128) + r * 128); }
+// Shared-memory operand descriptor in the 128-byte swizzle: 8-row groups `stride` bytes apart.  K-major
 // tiles have 64 elements of the inner dimension per row, the leading offset is not used; MN-major ones
 // (V) have 64 columns per row and find the next 64 columns `lead` bytes on.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((lead >> 4) & 0x3fffu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t stride, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)((lead >> 4) & 0x3fffu) << 16) |
+         ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// 16 bytes from global to shared memory (generic proxy); zeros when `live` is not set.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"((unsigned long long)src), "r"(live ? 16 : 0) : "memory");
 }
 // Instruction descriptor: f32 accumulators, f16 or bf16 operands, M = 128, N columns, B MN-major or K-major.
 __host__ __device__ constexpr uint32_t tc_idesc(bool bf16, int n, bool b_mn) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// Two floats in one instruction, and the largest of three.
+__device__ __forceinline__ void tc_fma2(float& x, float& y, float f, float g) {  // (x, y) = (x, y) * f + g
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(f), "f"(g));
+}
+__device__ __forceinline__ void tc_add2(float& x, float& y, float f, float g) {  // (x, y) += (f, g)
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(f), "f"(g));
+}
+__device__ __forceinline__ float tc_max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
 }
 
 template <bool BF16>
@@ -145,6 +190,51 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
   } else {
     return pack_half2(lo, hi);
+  }
+}
+
+// 128 rows of PIECES * 64 columns into a tile; row[i] of lane l is the offset of row 32 i + l's first column
+// (-1: zeros).  Pieces beyond a head's D columns belong to the next head.
+template <int PIECES, int D>
+__device__ __forceinline__ void tc_copy_rows(uint32_t dst, const __half* cache, const int64_t (&row)[4], int64_t head_stride,
+                                             int lane) {
+  constexpr int CH = PIECES * 8;  // 16-byte chunks, and lanes, of a row
+  constexpr int RPI = 32 / CH;    // rows of one warp-wide copy
+  const int c = lane % CH, rr = lane / CH, piece = c / 8;
+  const __half* mine = cache + (D == 64 && piece ? head_stride : 0) + (D == 64 ? c % 8 : c) * 8;
+#pragma unroll
+  for (int i = 0; i < 128 / RPI; ++i) {
+    const int r = i * RPI + rr;
+    const int64_t at = __shfl_sync(0xffffffffu, row[i * RPI / 32], r & 31);
+    cp_async16(dst + tc_row(r, piece) + (((c & 7) ^ (r & 7)) << 4), at >= 0 ? mine + at : cache, at >= 0);
+  }
+}
+
+// The same for pages of a multiple of 16 tokens: a piece of 16 tokens lies in one page, so its rows are a
+// stride apart.  `at` of lane g is the offset of token 16 g's row (-1: zeros), `live` tokens exist.
+template <int PIECES, int D>
+__device__ __forceinline__ void tc_copy_pages(uint32_t dst, const __half* cache, int64_t at, int64_t token_stride,
+                                              int64_t head_stride, int live, int lane) {
+  constexpr int CH = PIECES * 8, RPI = 32 / CH;
+  const int c = lane % CH, rr = lane / CH, piece = c / 8;
+  const __half* mine = cache + (D == 64 && piece ? head_stride : 0) + (D == 64 ? c % 8 : c) * 8 + rr * token_stride;
+  uint32_t to[8 / RPI];  // where the lane's rows of an 8-row group go
+#pragma unroll
+  for (int i = 0; i < 8 / RPI; ++i) {
+    const int r = i * RPI + rr;
+    to[i] = dst + tc_row(r, piece) + (((c & 7) ^ r) << 4);
+  }
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    const int64_t off = __shfl_sync(0xffffffffu, at, g);
+    const __half* src = off >= 0 ? mine + off : cache;
+    const int64_t step = off >= 0 ? RPI * token_stride : 0;
+    const int rows = off >= 0 ? live - 16 * g - rr : 0;  // of this lane: row i * RPI exists when below
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      cp_async16(to[i % (8 / RPI)] + (2 * g + i / (8 / RPI)) * 1024, src, i * RPI < rows);
+      src += step;
+    }
   }
 }
 
@@ -184,6 +274,20 @@ __device__ __forceinline__ bool tc_find_tile(const PrefillParams& a, int rows_pe
   return true;
 }
 
+// Unit `unit` of the loads: the first block's K tiles, then V of each block followed by the next one's K.
+template <int KT>
+__device__ __forceinline__ void tc_unit(int unit, int j0, int& j, int& k) {
+  if (unit < KT) {
+    j = j0;
+    k = unit;
+  } else {
+    const int u = unit - KT;
+    const int cyc = u / (KT + 1), in = u % (KT + 1);
+    j = j0 + cyc + (in ? 1 : 0);
+    k = in - 1;
+  }
+}
+
 // Keys that packed row r of the request sees.
 __device__ __forceinline__ int tc_limit(const TcTile& t, int r, int group) {
   const int n = t.len - t.tokens + r / group + 1;
@@ -209,16 +313,17 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   const uint32_t ring0 = base, q0 = base + C::NSLOT * C::SLOT;
   float* scales = reinterpret_cast<float*>(smem + C::NSLOT * C::SLOT + 2 * C::QTILE);
   uint8_t* misc = smem + C::NSLOT * C::SLOT + 2 * C::QTILE + C::SCALE_RING * C::SCALE_FLOATS * 4;
-  volatile int* meta = reinterpret_cast<volatile int*>(misc);               // bad 16-token pieces of a block
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 64);
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc + 68);
-  TcTile* tile_sh = reinterpret_cast<TcTile*>(misc + 96);
-  volatile int* have_tile = reinterpret_cast<volatile int*>(misc + 128);
-  const uint32_t bars = smem_u32(misc) + 256;
-  const uint32_t full0 = bars, empty0 = bars + 64, s_full = bars + 128, p_full = bars + 144, o_done = bars + 160,
-                 q_full = bars + 176, tail_bar = bars + 184, drain_bar = bars + 192;
-  float* squares = reinterpret_cast<float*>(misc + 512);  // [128] of the peer's half rows
-  static_assert(512 + 128 * 4 <= 2048, "misc area");
+  unsigned* meta = reinterpret_cast<unsigned*>(misc);  // [block mod 16][4]: its tokens whose page is not in the pool
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 256);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc + 260);
+  volatile int* have_tile = reinterpret_cast<volatile int*>(misc + 264);
+  TcTile* tile_sh = reinterpret_cast<TcTile*>(misc + 272);
+  const uint32_t bars = smem_u32(misc) + 320;
+  const uint32_t full0 = bars, empty0 = bars + 64, s_full = bars + 128, o_done = bars + 144, q_full = bars + 160,
+                 drain_bar = bars + 168, tail_bar = bars + 208, p_full = bars + 176;  // p_full: [tile][half of the keys]
+  float* squares = reinterpret_cast<float*>(misc + 640);  // [tile][128] of this CTA's columns, then of the peer's
+  float* weights = reinterpret_cast<float*>(misc + 640 + 2048);  // the norm's, of the slice
+  static_assert(kTcMetaRing * 16 <= 256 && (MAPS == 1 ? 640 : 640 + 2048 + 512) <= C::MISC, "misc area");
 
   // ---- which tile ------------------------------------------------------------------------------
   const int slice = C::SLICES == 1 ? 0 : blockIdx.x % C::SLICES;
@@ -228,28 +333,29 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   const int tile_no = tp.tiles - 1 - work % tp.tiles;  // a prompt's last tiles are its longest: they go first
   const int split = work / tp.tiles;
   if (warp == 0) {
+    if (lane < kTcMetaRing) *reinterpret_cast<uint4*>(meta + 4 * lane) = make_uint4(0, 0, 0, 0);
     TcTile t;
     const bool ok = tc_find_tile(a, C::ROWS, tile_no, lane, t);
     if (lane == 0) {
       *have_tile = ok ? 1 : 0;
       if (ok) *tile_sh = t;
       *abort_flag = 0;
-      for (int i = 0; i < kTcMetaRing; ++i) meta[i] = 0;
     }
   }
   if (warp == 8 && lane == 0) {
     for (int s = 0; s < C::NSLOT; ++s) {
-      mbar_init(full0 + 8 * s, C::WIDEN ? 128 : 1);
+      mbar_init(full0 + 8 * s, C::WIDEN ? 128 : 32);
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + 8 * t, 1);
-      mbar_init(p_full + 8 * t, 128);
+      mbar_init(p_full + 16 * t, 128);
+      mbar_init(p_full + 16 * t + 8, 128);
       mbar_init(o_done + 8 * t, 1);
     }
     mbar_init(q_full, 256);
-    mbar_init(tail_bar, 1);
     mbar_init(drain_bar, 1);
+    mbar_init(tail_bar, 1);
     fence_barrier_init();
     fence_proxy_async();
     if constexpr (!C::WIDEN) {
@@ -260,8 +366,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   __syncthreads();
   if (!*have_tile) return;  // the whole cluster has the same tile: nobody waits for this CTA
   // the peer runs before anything is written to its shared memory
-  if (C::SLICES == 2 && tp.splits == 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (C::SLICES == 2 && tp.splits == 1) tc_cluster_sync();
+  if (MAPS == 2 && tid < 128) weights[tid] = a.weight ? __ldg(a.weight + slice * C::DV + tid) : 1.f;
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((const void*)tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -287,94 +393,111 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     end[t] = max(j0, min(j1, (top + kTcBlock - 1) / kTcBlock));
   }
   const int jend = max(end[0], end[1]);
-  const int kv_end = tc_limit(tile, last_row, p.group);  // keys from here on are zero in shared memory
+  const int kv_end = tc_limit(tile, last_row, p.group);  // keys from here on are zeros in shared memory
 
-  // ================================ loader (16-bit pages) =============================================
-  if (warp == 8) {
+  // ================================ loaders (16-bit pages) =============================================
+  // V's tiles: warp 8; K's: warps 10 and 11 in turn.
+  if (warp == 8 || (!C::WIDEN && warp >= 10)) {
     if constexpr (!C::WIDEN) {
-      const int bt = tp.box_tokens, boxes = kTcBlock / bt;
-      int unit = 0;
-      bool tail_used = false;
-      // Unit order: K of the first block, then V of each block followed by K of the next.
       const int nb = jend - j0;
       const int units = nb > 0 ? nb * (C::KT + 1) : 0;
-      for (; unit < units; ++unit) {
-        // position in the cycle of V, K.. (the first block's K come ahead of it)
+      const bool whole = p.page % 16 == 0;                 // 16 tokens lie in one page
+      const bool by_tma = whole && (warp == 8 || p.page % 64 == 0);
+      const int bt = tp.box_tokens, boxes = kTcBlock / bt;
+      int turn = 0, issued = -1;
+      bool tail_used = false;
+      for (int unit = 0; unit < units; ++unit) {
         int j, k;  // block; K tile number or -1: V
-        if (unit < C::KT) {
-          j = j0;
-          k = unit;
-        } else {
-          const int u = unit - C::KT;
-          const int cyc = u / (C::KT + 1), in = u % (C::KT + 1);
-          j = j0 + cyc + (in ? 1 : 0);
-          k = in - 1;
-        }
+        tc_unit<C::KT>(unit, j0, j, k);
+        if (k < 0 ? warp != 8 : warp != 10 + (turn++ & 1)) continue;
         const int st = unit % C::NSLOT;
-        int ok = 1;
         const uint32_t dst = ring0 + st * C::SLOT;
-        const int token = j * kTcBlock + lane * bt;
-        int phys = p.num_blocks, off = 0, bad = 0;  // out of the map: zeros
-        if (lane < boxes && token < kv_end) {
-          const int page = token / p.page;
-          off = token - page * p.page;
-          const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
-          if ((unsigned)id < (unsigned)p.num_blocks) phys = id;
-          else {
-            if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
-            bad = ((1 << (bt / 16)) - 1) << (lane * bt / 16);
-          }
-        }
-        bad = __reduce_or_sync(kFull, (unsigned)bad);
-        // V rows from kv_end to the end of their box hold whatever the page holds: zero times that may be
-        // NaN, so they are cleared behind the copy
+        const int head0 = head * MAPS + (k < 0 ? slice * C::DV / D : k);
         const int live = kv_end - j * kTcBlock;  // keys of the block that exist
-        const bool tail = k < 0 && live < kTcBlock && live % bt != 0;
-        if (lane == 0) {
-          ok = mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag) ? 1 : 0;
-          if (ok) {
-            meta[j & (kTcMetaRing - 1)] = bad;
-            mbar_arrive_expect_tx(tail ? tail_bar : full0 + 8 * st, 128 * 2 * (k < 0 ? C::DV : D));
-          }
-        }
-        if (!__shfl_sync(kFull, ok, 0)) break;
-        if (lane < boxes) {
-          const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
-          const uint32_t at = dst + lane * bt * 128;
-          if (k >= 0) {
+        // One lane for each box (TMA), each 16 tokens, or each of four times 32 tokens: where their rows are.
+        int64_t row[4] = {-1, -1, -1, -1};
+        unsigned bad[4] = {0, 0, 0, 0};
+        int phys = p.num_blocks, off = 0;  // the block behind the last is out of the map: zeros
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(at + c * (128 * 128), &tm_k, bar, c * 64, off, head * MAPS + k, phys);
-          } else {
-#pragma unroll
-            for (int c = 0; c < C::DV / 64; ++c) {
-              const int col = slice * C::DV + c * 64;  // column of the pair's (or head's) V
-              tma_load_4d(at + c * (128 * 128), &tm_v, bar, col % D, off, head * MAPS + col / D, phys);
+        for (int i = 0; i < 4; ++i) {
+          if (whole && i) break;
+          const int in = by_tma ? lane * bt : whole ? 16 * lane : 32 * i + lane;
+          bool astray = false;
+          if (in < kTcBlock && in < live) {
+            const int token = j * kTcBlock + in, page = token / p.page;
+            const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
+            if ((unsigned)id < (unsigned)p.num_blocks) {
+              phys = id;
+              off = token - page * p.page;
+              row[i] = kv_row_offset(p, id, off, head0);
+            } else {
+              if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
+              astray = true;
             }
           }
+          bad[i] = __ballot_sync(kFull, astray);
         }
-        __syncwarp();
-        if (tail) {
-          tail_used = true;
-          int landed = 1;
-          if (lane == 0) landed = mbar_wait(tail_bar, 0, p.status, abort_flag) ? 1 : 0;  // the one tail of this CTA
-          if (!__shfl_sync(kFull, landed, 0)) {
-            ++unit;
-            break;
+        if (whole && bad[0]) {  // a bit a box or 16 tokens -> a bit a token
+          const unsigned pieces = bad[0];
+          const int each = by_tma ? bt : 16;
+          for (int i = 0; i < 4; ++i) {
+            bad[i] = 0;
+            for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / each)) & 1u) << e;
           }
-          const int to = (live / bt + 1) * bt;
-          for (int i = lane; i < (to - live) * (C::DV / 64) * 8; i += 32) {
-            const int r = live + i / 8 % (to - live), c = i / 8 / (to - live);
-            sts128(dst + c * (128 * 128) + r * 128 + (i & 7) * 16, make_uint4(0, 0, 0, 0));
-          }
-          fence_proxy_async();
+        }
+        if (!__all_sync(kFull, mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag))) break;
+        if (k == 0 && lane == 0)  // ahead of the block's scores
+          *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
+        if (by_tma) {
+          const bool tail = k < 0 && live < kTcBlock && live % bt != 0;  // V rows behind the last key in its box
+          const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
+          if (lane == 0) mbar_arrive_expect_tx(bar, 128 * 2 * (k < 0 ? C::DV : D));
+          if (lane > 0 && !tail) mbar_arrive(bar);
           __syncwarp();
-          if (lane == 0) mbar_arrive(full0 + 8 * st);
+          issued = unit;
+          if (lane < boxes) {
+            const uint32_t at = dst + lane * bt * 128;
+            if (k >= 0) {
+#pragma unroll
+              for (int c = 0; c < C::KH; ++c) tma_load_4d(at + c * (128 * 128), &tm_k, bar, c * 64, off, head0, phys);
+            } else {
+#pragma unroll
+              for (int c = 0; c < C::VC; ++c)
+                tma_load_4d(at + c * (128 * 128), &tm_v, bar, D == 64 ? 0 : c * 64, off, D == 64 ? head0 + c : head0, phys);
+            }
+          }
+          __syncwarp();
+          if (tail) {
+            tail_used = true;
+            if (!__all_sync(kFull, mbar_wait(tail_bar, 0, p.status, abort_flag))) break;  // the one tail of this CTA
+            const int to = (live / bt + 1) * bt;
+            for (int i = lane; i < (to - live) * C::VC * 8; i += 32) {
+              const int r = live + i / 8 % (to - live), c = i / 8 / (to - live);
+              sts128(dst + tc_row(r, c) + (i & 7) * 16, make_uint4(0, 0, 0, 0));
+            }
+            fence_proxy_async();
+            mbar_arrive(full0 + 8 * st);
+          }
+        } else {
+          if (whole) {
+            if (k < 0) tc_copy_pages<C::VC, D>(dst, (const __half*)p.v, row[0], p.kv_st, p.kv_sh, live, lane);
+            else tc_copy_pages<C::KH, D>(dst, (const __half*)p.k, row[0], p.kv_st, p.kv_sh, live, lane);
+          } else {
+            if (k < 0) tc_copy_rows<C::VC, D>(dst, (const __half*)p.v, row, p.kv_sh, lane);
+            else tc_copy_rows<C::KH, D>(dst, (const __half*)p.k, row, p.kv_sh, lane);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async();
+          mbar_arrive(full0 + 8 * st);
         }
       }
-      if (*abort_flag && lane == 0) {  // copies still in flight get a bounded chance to land
-        for (int k = 1; k <= C::NSLOT && k <= unit; ++k)
-          mbar_wait_slow(full0 + 8 * ((unit - k) % C::NSLOT), (uint32_t)((unit - k) / C::NSLOT) & 1u, nullptr, abort_flag, false);
+      if (*abort_flag && by_tma) {  // boxes still in flight get a bounded chance to land
+        for (int u = issued; u >= 0 && u > issued - C::NSLOT; --u) {
+          int j, k;
+          tc_unit<C::KT>(u, j0, j, k);
+          if ((k < 0) == (warp == 8))
+            mbar_wait_slow(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u, nullptr, abort_flag, false);
+        }
         if (tail_used) mbar_wait_slow(tail_bar, 0, nullptr, abort_flag, false);
       }
     }
@@ -389,19 +512,11 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       bool ok = true;
       for (int unit = 0; unit < units && ok; ++unit) {
         int j, k;
-        if (unit < C::KT) {
-          j = j0;
-          k = unit;
-        } else {
-          const int u = unit - C::KT;
-          const int cyc = u / (C::KT + 1), in = u % (C::KT + 1);
-          j = j0 + cyc + (in ? 1 : 0);
-          k = in - 1;
-        }
+        tc_unit<C::KT>(unit, j0, j, k);
         const int st = unit % C::NSLOT;
         const uint32_t dst = ring0 + st * C::SLOT;
         const int pieces = (k < 0 ? C::DV : D) / 16;  // of one row; a warp-wide load covers whole rows
-        if (k == 0 && me == 0) meta[(j + kTcMetaRing / 2) & (kTcMetaRing - 1)] = 0;  // read long ago, written far ahead
+        if (k == 0 && me < 4) meta[4 * ((j + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;  // read long ago, written far ahead
         uint4 x[kMaxChunk];
 #pragma unroll
         for (int i = 0; i < kMaxChunk; ++i) {
@@ -418,7 +533,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
               x[i] = __ldg(reinterpret_cast<const uint4*>((const char*)(k < 0 ? p.v : p.k) + at));
             } else {
               if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
-              atomicOr(const_cast<int*>(&meta[j & (kTcMetaRing - 1)]), 1 << (r / 16));
+              atomicOr(&meta[4 * (j & (kTcMetaRing - 1)) + r / 32], 1u << (r & 31));
             }
           }
         }
@@ -454,7 +569,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             h[2 * e] = cvt_pair<KV>(y, false);
             h[2 * e + 1] = cvt_pair<KV>(y, true);
           }
-          const uint32_t row = dst + (c / 4) * (128 * 128) + r * 128;
+          const uint32_t row = dst + tc_row(r, c / 4);
           const int ch = (2 * c) & 7;
           // neighbours that share banks store their two halves in opposite order
           const int flip = (c >> 2) & 1;
@@ -479,90 +594,118 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   }
   // ================================ matrix units ======================================================
   else if (warp == 9) {
-    if (lane == 0) {
-      constexpr uint32_t id_s = tc_idesc(C::BF16, 128, false);
-      constexpr uint32_t id_o = tc_idesc(C::BF16, C::DV / C::NP, true);
-      int unit = 0;
-      bool ok = true;
-      auto wait_unit = [&](int u) { return mbar_wait(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u, p.status, abort_flag); };
-      auto scores = [&](int t, uint32_t kslot) {  // S_t = Q_t K^T
+    constexpr uint32_t id_s = tc_idesc(C::BF16, 128, false);
+    constexpr uint32_t id_o = tc_idesc(C::BF16, C::DV / C::NP, true);
+    uint32_t mine;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(mine));
+    bool ok = true;
+    // every lane waits (the outcome is the warp's: all see the same phase or the same abort flag)
+    auto wait_bar = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(kFull, mbar_wait(bar, parity, p.status, abort_flag)) != 0;
+    };
+    auto scores = [&](int t, int kslot) {  // S_t = Q_t K^T
+      const uint64_t qd = tc_desc(q0 + t * C::QTILE, 1024, 0), kd = tc_desc(ring0 + kslot * C::SLOT, 1024, 0);
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
-          tc_mma_ss(tmem + t * 128, tc_desc(q0 + t * C::QTILE + off, 0), tc_desc(kslot + off, 0), id_s, ks > 0);
+      for (int ks = 0; ks < D / 16; ++ks)
+        tc_mma_ss(tmem + t * 128, qd + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4),
+                  kd + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4), id_s, ks > 0, mine);
+      tc_commit(s_full + 8 * t, mine);
+    };
+    auto values = [&](int t, int vslot, bool first, int half) {  // O_t (+)= P_t V, 64 keys
+      const uint64_t vd = tc_desc(ring0 + vslot * C::SLOT, 1024, 128 * 128);
+#pragma unroll
+      for (int z = 0; z < C::NP; ++z) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int ks = 4 * half + k;
+          const uint32_t pa = C::NP == 1 ? 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks % 2);
+          tc_mma_ts(tmem + 256 + t * 128 + z * 64, tmem + t * 128 + pa, vd + ((z * (128 * 128) + ks * 2048) >> 4), id_o,
+                    !first || ks > 0, mine);
         }
-        tc_commit(s_full + 8 * t);
+      }
+    };
+    if (jend > j0) {
+      ok = wait_bar(q_full, 0);
+      // unit u lives in slot u % NSLOT; slot and phase of the next unit are counted along
+      int slot = 0;
+      uint32_t phase = 0;
+      auto step = [&] {
+        if (++slot == C::NSLOT) {
+          slot = 0;
+          phase ^= 1;
+        }
       };
-      auto values = [&](int t, uint32_t vslot, bool first) {  // O_t (+)= P_t V
+      // the first block's scores
+      if (ok) ok = wait_bar(full0, 0);
+      if (ok) {
+        tc_fence_after();
+        if (end[0] > j0) scores(0, 0);
+        step();
+        if constexpr (MAPS == 2) {
+          ok = wait_bar(full0 + 8, 0);
+          if (ok) {
+            tc_fence_after();
+            scores(1, 1);
+            tc_commit(empty0, mine);
+            tc_commit(empty0 + 8, mine);
+          }
+          step();
+        } else {
+          if (end[1] > j0) scores(1, 0);
+          tc_commit(empty0, mine);
+        }
+      }
+      for (int j = j0; j < jend && ok; ++j) {
+        const uint32_t par = (uint32_t)(j - j0) & 1u;
+        const bool more = j + 1 < jend;
+        const int vslot = slot;
+        const uint32_t vphase = phase;
+        int kslot[C::KT];
+        uint32_t kphase[C::KT];
+        step();
+        if (more) {
 #pragma unroll
-        for (int z = 0; z < C::NP; ++z) {
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            const uint32_t pa = C::NP == 1 ? 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks % 2);
-            tc_mma_ts(tmem + 256 + t * 128 + z * 64, tmem + t * 128 + pa,
-                      tc_desc(vslot + z * (128 * 128) + ks * 2048, 128 * 128), id_o, !first || ks > 0);
+          for (int k = 0; k < C::KT; ++k) {
+            kslot[k] = slot;
+            kphase[k] = phase;
+            step();
           }
         }
-      };
-      if (jend > j0) {
-        ok = mbar_wait(q_full, 0, p.status, abort_flag);
-        // the first block's scores
-        if (ok) ok = wait_unit(0);
-        if (ok) {
-          tc_fence_after();
-          if (end[0] > j0) scores(0, ring0);
-          if constexpr (MAPS == 2) {
-            ok = wait_unit(1);
-            tc_fence_after();
-            if (ok) {
-              scores(1, ring0 + (1 % C::NSLOT) * C::SLOT);
-              tc_commit(empty0);
-              tc_commit(empty0 + 8);
-            }
-          } else {
-            if (end[1] > j0) scores(1, ring0);
-            tc_commit(empty0);
-          }
-        }
-        unit = C::KT;
-        for (int j = j0; j < jend && ok; ++j) {
-          const int vs = unit % C::NSLOT;
-          const bool more = j + 1 < jend;
-          bool have_v = false, have_k = false;
+        ok = wait_bar(full0 + 8 * vslot, vphase);
+        if (more && C::KT == 1 && ok) ok = wait_bar(full0 + 8 * kslot[0], kphase[0]);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= end[t] || !ok) continue;
-            ok = mbar_wait(p_full + 8 * t, (uint32_t)(j - j0) & 1u, p.status, abort_flag);
-            if (ok && !have_v) ok = wait_unit(unit);
-            if (!ok) break;
-            have_v = true;
-            tc_fence_after();
-            values(t, ring0 + vs * C::SLOT, j == j0);
-            if (j + 1 < end[t]) {
-              const int ku = unit + 1 + (MAPS == 2 ? t : 0);
-              if (MAPS == 2 || !have_k) ok = wait_unit(ku);
-              if (!ok) break;
-              have_k = true;
-              tc_fence_after();
-              scores(t, ring0 + (ku % C::NSLOT) * C::SLOT);
-            } else {
-              tc_commit(o_done + 8 * t);
-            }
-          }
+        for (int t = 0; t < 2; ++t) {
+          if (j >= end[t] || !ok) continue;
+          ok = wait_bar(p_full + 16 * t, par);
           if (!ok) break;
-          // both tiles' products with these tiles are issued: their slots are free when they are done
-          tc_commit(empty0 + 8 * vs);
-          ++unit;
-          if (more) {
-#pragma unroll
-            for (int k = 0; k < C::KT; ++k) tc_commit(empty0 + 8 * ((unit + k) % C::NSLOT));
-            unit += C::KT;
+          tc_fence_after();
+          values(t, vslot, j == j0, 0);
+          ok = wait_bar(p_full + 16 * t + 8, par);
+          if (!ok) break;
+          tc_fence_after();
+          values(t, vslot, j == j0, 1);
+          if (j + 1 < end[t]) {
+            if constexpr (C::KT == 2) {
+              ok = wait_bar(full0 + 8 * kslot[t], kphase[t]);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            scores(t, kslot[C::KT == 2 ? t : 0]);
+          } else {
+            tc_commit(o_done + 8 * t, mine);
           }
         }
-        if (!ok) {  // products in flight get a bounded chance to end before tensor memory is freed
-          tc_commit(drain_bar);
-          mbar_wait_slow(drain_bar, 0, nullptr, abort_flag, false);
+        if (!ok) break;
+        // both tiles' products with these tiles are issued: their slots are free when they are done
+        tc_commit(empty0 + 8 * vslot, mine);
+        if (more) {
+#pragma unroll
+          for (int k = 0; k < C::KT; ++k) tc_commit(empty0 + 8 * kslot[k], mine);
         }
+      }
+      if (!ok) {  // products in flight get a bounded chance to end before tensor memory is freed
+        tc_commit(drain_bar, mine);
+        mbar_wait_slow(drain_bar, 0, nullptr, abort_flag, false);
       }
     }
     __syncwarp();
@@ -578,20 +721,24 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
 
     // ---- Q into shared memory, 16 bytes at a time, in the 128-byte swizzle --------------------------
     if (jend > j0) {
-      constexpr int CH = D / 8;  // pieces of a row
-#pragma unroll 4
-      for (int i = me; i < 128 * CH; i += 128) {
-        const int r = i / CH, c = i % CH;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < n_rows) {
-          const int pr = first_row + r;
-          const int tok = pr / p.group, g = pr - tok * p.group;
-          const int64_t at = (int64_t)(tile.first_token + tok) * p.q_sb + (int64_t)(head * p.group + g) * p.q_sh +
-                             (MAPS == 2 ? t * a.q_sm : 0) + c * 8;
-          x = __ldg(reinterpret_cast<const uint4*>((const __half*)p.q + at));
+      constexpr int CH = D / 8;         // 16-byte chunks of a row
+      constexpr int RPI = 128 / CH;     // rows of one round of the tile's threads
+      const int c = me % CH, rr = me / CH;
+      int tok = (first_row + rr) / p.group, g = (first_row + rr) - tok * p.group;
+#pragma unroll
+      for (int i = 0; i < 128 / RPI; ++i) {
+        const int r = i * RPI + rr;
+        const int64_t at = (int64_t)(tile.first_token + tok) * p.q_sb + (int64_t)(head * p.group + g) * p.q_sh +
+                           (MAPS == 2 ? t * a.q_sm : 0) + c * 8;
+        cp_async16(q0 + t * C::QTILE + tc_row(r, c / 8) + (((c & 7) ^ (r & 7)) << 4),
+                   r < n_rows ? (const __half*)p.q + at : (const __half*)p.q, r < n_rows);
+        g += RPI;
+        while (g >= p.group) {
+          g -= p.group;
+          ++tok;
         }
-        sts128(q0 + t * C::QTILE + (c / 8) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), x);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async();
       mbar_arrive(q_full);
     }
@@ -604,8 +751,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       ok = mbar_wait(s_full + 8 * t, (uint32_t)(j - j0) & 1u, p.status, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const int bad = meta[j & (kTcMetaRing - 1)];
-      const bool masked = (j + 1) * kTcBlock > least || bad;
+      const volatile unsigned* bad = meta + 4 * (j & (kTcMetaRing - 1));
+      const bool masked = (j + 1) * kTcBlock > least || (bad[0] | bad[1] | bad[2] | bad[3]);
       const int room = limit - j * kTcBlock;  // columns below this one are seen
       const float* ks = SCALED ? scales + (j % C::SCALE_RING) * C::SCALE_FLOATS + (MAPS == 2 ? t * 128 : 0) : nullptr;
       const float* vs = SCALED ? scales + (j % C::SCALE_RING) * C::SCALE_FLOATS + C::KT * 128 : nullptr;
@@ -622,9 +769,10 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           }
         }
         if (masked) {
+          const unsigned astray = bad[c0 / 32];
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (c0 + c >= room || ((bad >> ((c0 + c) / 16)) & 1)) x[c] = -INFINITY;
+            if (c0 + c >= room || ((astray >> c) & 1)) x[c] = -INFINITY;
         }
       };
       // The row's maximum; 16-bit pages keep the 128 scores in registers, 8-bit ones (more warps, fewer
@@ -646,7 +794,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         }
         shape_scores(y, c0);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], y[c]);
+        for (int c = 0; c < 32; c += 2) mx[(c >> 1) & 3] = tc_max3(mx[(c >> 1) & 3], y[c], y[c + 1]);
       }
       const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
       if (j == j0) {
@@ -677,9 +825,11 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           shape_scores(y, c0);
         }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          y[c] = fast_exp2(fmaf(y[c], p.scale_log2, -from));
-          sum[c & 3] += y[c];
+        for (int c = 0; c < 32; c += 2) {
+          tc_fma2(y[c], y[c + 1], p.scale_log2, -from);
+          y[c] = fast_exp2(y[c]);
+          y[c + 1] = fast_exp2(y[c + 1]);
+          tc_add2(sum[c & 2], sum[(c & 2) + 1], y[c], y[c + 1]);
         }
         uint32_t pk[16];
 #pragma unroll
@@ -698,15 +848,18 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           // columns below 16 (or 32) * (c0 / 32 + 1) hold scores that have been read
           tc_st16(s_at + (C::NP == 1 ? c0 / 2 : c0 + 16 * z), pk);
         }
+        if (c0 & 32) {  // half of the keys: the product with V may begin on them
+          tc_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_full + 16 * t + 8 * (c0 / 64));
+        }
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tc_wait_st();
-      tc_fence_before();
-      mbar_arrive(p_full + 8 * t);
     }
 
     // ---- results ----------------------------------------------------------------------------------------
-    if (ok && end[t] > j0) ok = mbar_wait(o_done + 8 * t, 0, p.status, abort_flag);
+    // (maps = 2: both tiles' products, of which the second tile's are the last: the ring is written below)
+    if (ok && end[t] > j0) ok = mbar_wait(o_done + 8 * (MAPS == 2 ? 1 : t), 0, p.status, abort_flag);
     tc_fence_after();
     const bool any = end[t] > j0;  // else tensor memory holds nothing of this tile
     const float inv = l > 0.f || l != l ? 1.f / (l * kBoost) : 0.f;
@@ -758,96 +911,67 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         }
       }
     } else {
-      // The second map's rows reach the first map's threads through the ring (every tile in it has been
-      // read), a column of 128 rows at a time: neighbouring lanes, neighbouring words.
-      float* pass = reinterpret_cast<float*>(smem);
+      // A row's two maps are in two threads.  Through the ring (every tile in it has been read) the first map's
+      // thread gets the second's columns 0..63 and gives its own 64..127, a column of 128 rows at a time:
+      // neighbouring lanes, neighbouring words.  Each then has 64 columns of the difference in registers.
+      float* pass = reinterpret_cast<float*>(smem) + t * (64 * 128);        // what this thread gives
+      const float* take = reinterpret_cast<const float*>(smem) + (t ^ 1) * (64 * 128);
       static_assert(C::NSLOT * C::SLOT >= 128 * 128 * 4, "room for one tile of f32");
-      const float lam = a.lambda(row, hq);
-      if (t == 1) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          float o[32];
-          if (any) {
-            tc_ld32(o_at + c0, o);
-            tc_wait_ld();
-          }
+      const float mult = inv != 0.f && any ? (t == 0 ? inv : inv * a.lambda(row, hq)) : 0.f;
+      float x[64];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) pass[(c0 + c) * 128 + me] = any && inv != 0.f ? o[c] * inv * lam : 0.f;
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        float o[32];
+        if (any) {
+          tc_ld32(o_at + c0, o);
+          tc_wait_ld();
+        }
+        const bool mine = (c0 < 64) == (t == 0);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float y = mult != 0.f ? o[c] * mult : 0.f;
+          if (!mine) pass[((c0 & 32) + c) * 128 + me] = y;
+          else x[(c0 & 32) + c] = y;
         }
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       float square = 0.f;
-      if (t == 0) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          float o[32];
-          if (any) {
-            tc_ld32(o_at + c0, o);
-            tc_wait_ld();
-          }
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const float y = (any && inv != 0.f ? o[c] * inv : 0.f) - pass[(c0 + c) * 128 + me];
-            pass[(c0 + c) * 128 + me] = y;
-            square = fmaf(y, y, square);
-          }
-        }
+      for (int c = 0; c < 64; ++c) {
+        const float y = take[c * 128 + me];
+        x[c] = t == 0 ? x[c] - y : y - x[c];
+        square = fmaf(x[c], x[c], square);
       }
-      if constexpr (C::SLICES == 2) {
-        if (t == 0) {  // this half's sum of squares to the other half's CTA
-          uint32_t peer;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(squares + me)), "r"(slice ^ 1));
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer), "f"(square) : "memory");
-        }
+      squares[t * 128 + me] = square;
+      if constexpr (C::SLICES == 2) {  // the other half of V's columns is in the other CTA of the cluster
+        uint32_t peer;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(smem_u32(squares + 256 + t * 128 + me)), "r"(slice ^ 1));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(peer), "f"(square) : "memory");
+        tc_cluster_sync();
+      } else {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      // with two slices the store waits for the cluster (below)
-      if constexpr (C::SLICES == 1) {
-        if (t == 0 && live && ok) {
-          float factor = a.out_scale;
-          if (a.norm) factor *= rsqrtf(square * (1.f / (MAPS * D)) + a.eps);
-          uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh);
-#pragma unroll 4
-          for (int c = 0; c < 128; c += 8) {
-            float y[8];
+      if (live && ok) {
+        float total = squares[me] + squares[128 + me];
+        if constexpr (C::SLICES == 2) total += squares[256 + me] + squares[384 + me];
+        float factor = a.out_scale;
+        if (a.norm) factor *= rsqrtf(total * (1.f / (MAPS * D)) + a.eps);
+        const int col = slice * C::DV + t * 64;
+        uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh + col);
+        const float* wt = weights + t * 64;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = pass[(c + e) * 128 + me] * factor * (a.weight ? __ldg(a.weight + c + e) : 1.f);
-            dst[c / 8] = make_uint4(tc_pack<C::BF16>(y[0], y[1]), tc_pack<C::BF16>(y[2], y[3]), tc_pack<C::BF16>(y[4], y[5]),
-                                    tc_pack<C::BF16>(y[6], y[7]));
-          }
+        for (int c = 0; c < 64; c += 8) {
+          const float4 w0 = *reinterpret_cast<const float4*>(wt + c), w1 = *reinterpret_cast<const float4*>(wt + c + 4);
+          dst[c / 8] = make_uint4(tc_pack<C::BF16>(x[c] * factor * w0.x, x[c + 1] * factor * w0.y),
+                                  tc_pack<C::BF16>(x[c + 2] * factor * w0.z, x[c + 3] * factor * w0.w),
+                                  tc_pack<C::BF16>(x[c + 4] * factor * w1.x, x[c + 5] * factor * w1.y),
+                                  tc_pack<C::BF16>(x[c + 6] * factor * w1.z, x[c + 7] * factor * w1.w));
         }
       }
     }
   }
-  // ---- the other half's sums of squares (head_dim 128, maps = 2) --------------------------------------------
-  if constexpr (C::SLICES == 2) {
-    if (tp.splits == 1) {
-      __syncthreads();
-      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-      if (warp < 4) {
-        const int me = tid;
-        const bool live = me < tile.count && !*abort_flag;
-        if (live) {
-          const int pr = tile.row0 + me, tok = pr / p.group, hq = head * p.group + pr - tok * p.group;
-          const float* pass = reinterpret_cast<const float*>(smem);
-          const int64_t row = tile.first_token + tok;
-          float own = 0.f;
-          for (int c = 0; c < 128; ++c) own = fmaf(pass[c * 128 + me], pass[c * 128 + me], own);
-          float factor = a.out_scale;
-          if (a.norm) factor *= rsqrtf((own + squares[me]) * (1.f / (MAPS * D)) + a.eps);
-          uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh + slice * 128);
-#pragma unroll 4
-          for (int c = 0; c < 128; c += 8) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              y[e] = pass[(c + e) * 128 + me] * factor * (a.weight ? __ldg(a.weight + slice * 128 + c + e) : 1.f);
-            dst[c / 8] = make_uint4(tc_pack<C::BF16>(y[0], y[1]), tc_pack<C::BF16>(y[2], y[3]), tc_pack<C::BF16>(y[4], y[5]),
-                                    tc_pack<C::BF16>(y[6], y[7]));
-          }
-        }
-      }
-    }
-  }
+  // the warps that are not part of the exchange of sums arrive for it here
+  if (C::SLICES == 2 && tp.splits == 1 && warp >= 8) tc_cluster_sync();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {

@@ -22,9 +22,8 @@ __host__ inline TcShape tc_shape(int head_dim, int maps) {
   return s;
 }
 
-#define PD_TC_LAUNCHER(name)                                                                                     \
-  cudaError_t name(int head_dim, int maps, const TcParams& tp, const CUtensorMap& mk, const CUtensorMap& mv,     \
-                   unsigned grid, cudaStream_t st)
+#define PD_TC_LAUNCHER(name) \
+  cudaError_t name(int head_dim, int maps, const TcParams& tp, const CUtensorMap& mk, const CUtensorMap& mv, unsigned grid, cudaStream_t st)
 PD_TC_LAUNCHER(tc_launch_f16);
 PD_TC_LAUNCHER(tc_launch_bf16);
 PD_TC_LAUNCHER(tc_launch_e5m2);

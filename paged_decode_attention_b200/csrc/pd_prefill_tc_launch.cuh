@@ -7,8 +7,8 @@
 namespace pd {
 
 template <int KV, int D, int MAPS, bool SCALED>
-static inline cudaError_t tc_launch_one(const TcParams& tp, const CUtensorMap& mk, const CUtensorMap& mv, unsigned grid,
-                                        cudaStream_t st) {
+static inline cudaError_t tc_launch_one(const TcParams& tp, const CUtensorMap& mk, const CUtensorMap& mv,
+                                    unsigned grid, cudaStream_t st) {
   using C = TcCfg<KV, D, MAPS, SCALED>;
   auto* kern = tc_prefill_kernel<KV, D, MAPS, SCALED>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);

@@ -131,16 +131,16 @@ def test_prefill_lengths(maps, lens, new):
     both(ref.make(lens, new, heads=4, kv_heads=2, dim=128, kv="bf16", maps=maps, seed=sum(lens)), "stream")
 
 
-@pytest.mark.parametrize("page", [16, 32, 48, 64, 128, 256])
+@pytest.mark.parametrize("page", [1, 5, 16, 32, 48, 128, 256, 500])
 @pytest.mark.parametrize("kv", ["fp16", "fp8_e5m2"])
 def test_prefill_pages(page, kv):
-    both(ref.make([1, page - 1, page, page + 1, 3 * page + 5], [1, page - 1, 3, page + 1, 2 * page], heads=4, kv_heads=2,
+    both(ref.make([1, page - 1, page, page + 1, 3 * page + 5], [1, page - 1, 1, page + 1, 2 * page], heads=4, kv_heads=2,
                   page=page, kv=kv), "stream")
 
 
 @pytest.mark.parametrize("maps", [1, 2])
-@pytest.mark.parametrize("dim,page,kv,io", [(32, 16, "fp16", None), (256, 16, "bf16", None), (64, 5, "int8", None),
-                                            (64, 16, "fp16", torch.bfloat16), (128, 16, "bf16", torch.float16), (32, 16, "int8", None)])
+@pytest.mark.parametrize("dim,page,kv,io", [(32, 16, "fp16", None), (256, 16, "bf16", None), (64, 16, "fp16", torch.bfloat16),
+                                            (128, 16, "bf16", torch.float16), (32, 16, "int8", None)])
 def test_prefill_on_the_general_kernel(maps, dim, page, kv, io):
     both(ref.make([30, 40, 133], [30, 4, 20], heads=3, kv_heads=1, dim=dim, page=page, kv=kv, io=io, maps=maps), "simple")
 
@@ -165,9 +165,12 @@ def test_rows_of_nobody_are_left_as_they_were(maps, kernel):
 
 
 @pytest.mark.parametrize("kernel", ["simple", "auto"])
-def test_prefill_bad_blocks_are_left_out_and_flagged(kernel):
+@pytest.mark.parametrize("kv,page", [("fp16", 16), ("bf16", 5), ("int8", 16), ("fp8_e5m2", 7)])
+def test_prefill_bad_blocks_are_left_out_and_flagged(kernel, kv, page):
+    """The last of the lengths passes more blocks than the kernel keeps masks of."""
     for maps in (1, 2):
-        c = ref.make([300, 64], [300, 10], heads=4, kv_heads=2, dim=64, maps=maps)
+        c = ref.make([300, 64, 2500], [300, 10, 20], heads=4, kv_heads=2, dim=64, kv=kv, page=page, maps=maps)
+        c.cache.block_table[2, 1] = -3
         c.cache.block_table[0, 3] = 10 ** 6
         c.cache.block_table[1, 0] = -1
         status = torch.zeros(1, dtype=torch.int32, device="cuda")
