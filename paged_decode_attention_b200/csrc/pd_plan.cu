@@ -20,7 +20,11 @@ namespace pd {
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxBatch = 8192;
 constexpr int kPlanMaxCtas = 8;
-constexpr int kPlanRun = 4;  // consecutive tokens of one thread: one search, one or two block ids, 16-byte stores
+// Consecutive tokens of one thread.  Up to a token for every thread there can be it is one: their block ids
+// are then fetched side by side (256 requests with a token each: four a thread took 9.9 us, the chain of
+// their four loads).  Above, four share a search and mostly a block id and are stored 16 bytes at a time.
+constexpr int kPlanRunMany = 4;
+constexpr int kPlanFewTokens = kPlanThreads * kPlanMaxCtas;
 
 struct PlanParams {
   int32_t* table;
@@ -46,6 +50,7 @@ struct PlanRow {
 
 __device__ __forceinline__ int plan_pages(int64_t tokens, int page) { return (int)((tokens + page - 1) / page); }
 
+template <int kPlanRun>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   extern __shared__ PlanRow rows[];  // batch + 1: the last holds the totals
   __shared__ long long warp_sum[kPlanThreads / 32];
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   __syncthreads();
   const int total = rows[p.batch].start;
 
-  // ---- slots and positions: four consecutive tokens a thread -------------------------------------
+  // ---- slots and positions: kPlanRun consecutive tokens a thread ----------------------------------
   const int64_t runs = ((int64_t)p.tokens + kPlanRun - 1) / kPlanRun;
   for (int64_t r = (int64_t)cta * kPlanThreads + tid; r < runs; r += (int64_t)ctas * kPlanThreads) {
     const int t0 = (int)(r * kPlanRun);
@@ -145,9 +150,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
         }
       }
     }
-    if (p.wide && t0 + kPlanRun <= p.tokens) {
+    if (kPlanRun % 2 == 0 && p.wide && t0 + kPlanRun <= p.tokens) {
 #pragma unroll
-      for (int k = 0; k < kPlanRun; k += 2) {
+      for (int k = 0; k + 1 < kPlanRun; k += 2) {
         *reinterpret_cast<longlong2*>(p.slots + t0 + k) = make_longlong2(slot[k], slot[k + 1]);
         *reinterpret_cast<longlong2*>(p.positions + t0 + k) = make_longlong2(pos[k], pos[k + 1]);
       }
@@ -215,12 +220,14 @@ extern "C" PD_API int pd_plan_step(const PdPlanArgs* a) {
   p.tokens = a->num_tokens;
   p.wide = ((uintptr_t)a->slot_mapping % 16 == 0 && (uintptr_t)a->positions % 16 == 0) ? 1 : 0;
   p.status = a->status;
-  // one CTA up to a run of four tokens a thread; the cluster barrier costs less than a second round
+  const bool few = a->num_tokens <= kPlanFewTokens;
+  auto* kern = few ? plan_kernel<1> : plan_kernel<kPlanRunMany>;
+  // as many CTAs as give every thread its run, up to the cluster's eight
   int ctas = 1;
-  while (ctas < kPlanMaxCtas && (int64_t)ctas * kPlanThreads * kPlanRun < a->num_tokens) ctas <<= 1;
+  while (ctas < kPlanMaxCtas && (int64_t)ctas * kPlanThreads * (few ? 1 : kPlanRunMany) < a->num_tokens) ctas <<= 1;
   const size_t smem = (size_t)(a->batch + 1) * sizeof(PlanRow);
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            (int)((kPlanMaxBatch + 1) * sizeof(PlanRow))) != cudaSuccess)
     return PD_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -234,6 +241,6 @@ extern "C" PD_API int pd_plan_step(const PdPlanArgs* a) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, plan_kernel, p) == cudaSuccess ? PD_OK : PD_ERR_CUDA;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? PD_OK : PD_ERR_CUDA;
 }

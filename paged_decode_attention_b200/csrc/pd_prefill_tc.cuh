@@ -503,49 +503,62 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     }
   }
   // ================================ widening warps (8-bit pages) =======================================
+  // Four warps; a thread takes 16-byte pieces me, me + 128, .. of a tile's rows.  The pieces of the next unit
+  // are on their way while this one's are widened and stored, and the block ids of a block are fetched a
+  // block ahead (without that a tile cost two round trips to memory).
   else if (warp >= 10) {
     if constexpr (C::WIDEN) {
       const int me = tid - 320;  // 0 .. 127
-      constexpr int kMaxChunk = (D > C::DV ? D : C::DV) / 16;  // 16-byte pieces of a row = pieces per thread and tile
+      constexpr int PK = D / 16, PV = C::DV / 16;        // 16-byte pieces of a K and of a V row = of a thread
+      constexpr int PM = PK > PV ? PK : PV;
       const int nb = jend - j0;
       const int units = nb > 0 ? nb * (C::KT + 1) : 0;
-      bool ok = true;
-      for (int unit = 0; unit < units && ok; ++unit) {
-        int j, k;
-        tc_unit<C::KT>(unit, j0, j, k);
-        const int st = unit % C::NSLOT;
-        const uint32_t dst = ring0 + st * C::SLOT;
-        const int pieces = (k < 0 ? C::DV : D) / 16;  // of one row; a warp-wide load covers whole rows
-        if (k == 0 && me < 4) meta[4 * ((j + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;  // read long ago, written far ahead
-        uint4 x[kMaxChunk];
+      const bool whole = p.page % 16 == 0;               // 16 tokens lie in one page
+      // lane l < 8: block id of tokens 16 l .. of block j (-1: none), and whether there should have been one
+      auto fetch_ids = [&](int j) {
+        const int token = j * kTcBlock + 16 * lane;
+        int id = -1;
+        if (whole && lane < 8 && token < kv_end) id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + token / p.page);
+        return id;
+      };
+      // offset of token r of block j in a cache tensor of kv head h, -1: no such key
+      auto place = [&](int ids, int j, int r, int& off) {
+        const int token = j * kTcBlock + r;
+        const int from = __shfl_sync(kFull, ids, r / 16);
+        off = 0;
+        if (token >= kv_end) return -1;
+        const int page = token / p.page;
+        const int id = whole ? from : __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
+        off = token - page * p.page;
+        if ((unsigned)id < (unsigned)p.num_blocks) return id;
+        if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
+        atomicOr(&meta[4 * (j & (kTcMetaRing - 1)) + r / 32], 1u << (r & 31));
+        return -1;
+      };
+      auto fetch = [&](int j, int k, int ids, uint4 (&x)[PM], float (&sc)[SCALED ? C::KT + C::VH : 1]) {
+        const int pieces = k < 0 ? PV : PK;
 #pragma unroll
-        for (int i = 0; i < kMaxChunk; ++i) {
+        for (int i = 0; i < PM; ++i) {
           x[i] = make_uint4(0, 0, 0, 0);
-          const int n = me + i * 128;
-          const int r = n / pieces, c = n % pieces;
-          const int token = j * kTcBlock + r;
-          if (i < pieces && token < kv_end) {
-            const int page = token / p.page;
-            const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
-            if ((unsigned)id < (unsigned)p.num_blocks) {
-              const int col = k < 0 ? slice * C::DV + c * 16 : c * 16;
-              const int64_t at = kv_row_offset(p, id, token - page * p.page, head * MAPS + (k < 0 ? col / D : k)) + col % D;
-              x[i] = __ldg(reinterpret_cast<const uint4*>((const char*)(k < 0 ? p.v : p.k) + at));
-            } else {
-              if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
-              atomicOr(&meta[4 * (j & (kTcMetaRing - 1)) + r / 32], 1u << (r & 31));
-            }
+          if (i >= pieces) continue;
+          const int n = me + i * 128, r = n / pieces, c = n % pieces;
+          int off;
+          const int id = place(ids, j, r, off);
+          if (id >= 0) {
+            const int col = k < 0 ? slice * C::DV + c * 16 : c * 16;
+            const int64_t at = kv_row_offset(p, id, off, head * MAPS + (k < 0 ? col / D : k)) + col % D;
+            x[i] = __ldg(reinterpret_cast<const uint4*>((const char*)(k < 0 ? p.v : p.k) + at));
           }
         }
-        // the block's scales, K's and V's, with its first K tile: the softmax needs them ahead of V itself
-        float sc[SCALED ? C::KT + C::VH : 1] = {};
         if constexpr (SCALED) {
-          const int token = j * kTcBlock + me;
-          if (k == 0 && token < kv_end) {
-            const int page = token / p.page;
-            const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
-            if ((unsigned)id < (unsigned)p.num_blocks) {
-              const int64_t at = scale_offset(p, id, token - page * p.page, head * MAPS);
+          // the block's scales, K's and V's, with its first K tile: the softmax needs them ahead of V itself
+          if (k == 0) {
+            int off;
+            const int id = place(ids, j, me, off);
+#pragma unroll
+            for (int z = 0; z < C::KT + C::VH; ++z) sc[z] = 0.f;
+            if (id >= 0) {
+              const int64_t at = scale_offset(p, id, off, head * MAPS);
 #pragma unroll
               for (int z = 0; z < C::KT; ++z) sc[z] = __half2float(__ldg(p.k_scale + at + z));
 #pragma unroll
@@ -554,13 +567,39 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             }
           }
         }
-        ok = mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag);
+      };
+      int ids = fetch_ids(j0), ids_next = fetch_ids(j0 + 1);  // of block idj and the one behind it
+      int idj = j0;
+      uint4 x[PM];
+      float sc[SCALED ? C::KT + C::VH : 1];
+      if (units > 0) fetch(j0, 0, ids, x, sc);
+      bool ok = true;
+      for (int unit = 0; unit < units && ok; ++unit) {
+        int j, k;
+        tc_unit<C::KT>(unit, j0, j, k);
+        uint4 nx[PM];
+        float nsc[SCALED ? C::KT + C::VH : 1];
+        if (unit + 1 < units) {
+          int j2, k2;
+          tc_unit<C::KT>(unit + 1, j0, j2, k2);
+          if (k2 == 0 && me < 4) meta[4 * ((j2 + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;  // read long ago, written far ahead
+          // a block's V comes behind its K, the next block's K behind that: its ids are fetched with this V
+          if (j2 > idj && k2 < 0) {
+            ids = ids_next;
+            ++idj;
+            ids_next = fetch_ids(idj + 1);
+          }
+          fetch(j2, k2, j2 > idj ? ids_next : ids, nx, nsc);
+        }
+        const int st = unit % C::NSLOT;
+        const uint32_t dst = ring0 + st * C::SLOT;
+        ok = __all_sync(kFull, mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag));
         if (!ok) break;
+        const int pieces = k < 0 ? PV : PK;
 #pragma unroll
-        for (int i = 0; i < kMaxChunk; ++i) {
+        for (int i = 0; i < PM; ++i) {
           if (i >= pieces) continue;
-          const int n = me + i * 128;
-          const int r = n / pieces, c = n % pieces;
+          const int n = me + i * 128, r = n / pieces, c = n % pieces;
           const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
           uint32_t h[8];
 #pragma unroll
@@ -575,9 +614,9 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           const int flip = (c >> 2) & 1;
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
-            const int half = o ^ flip;
-            const uint4 y = half ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
-            sts128(row + (((ch + half) ^ (r & 7)) << 4), y);
+            const bool upper = (o ^ flip) != 0;
+            const uint4 y = make_uint4(upper ? h[4] : h[0], upper ? h[5] : h[1], upper ? h[6] : h[2], upper ? h[7] : h[3]);
+            sts128(row + (((ch + (upper ? 1 : 0)) ^ (r & 7)) << 4), y);
           }
         }
         if constexpr (SCALED) {
@@ -589,6 +628,12 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         }
         fence_proxy_async();
         mbar_arrive(full0 + 8 * st);
+#pragma unroll
+        for (int i = 0; i < PM; ++i) x[i] = nx[i];
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int z = 0; z < C::KT + C::VH; ++z) sc[z] = nsc[z];
+        }
       }
     }
   }

@@ -81,6 +81,19 @@ def _call_on_device(device: torch.device, fn, *fn_args) -> int:
         return fn(*fn_args)
 
 
+def _current_stream(index: int) -> int:
+    """The current stream of device `index` as the integer the C ABI takes, without a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _call_on_index(index: int, fn, *fn_args) -> int:
+    """``_call_on_device`` for a device index."""
+    if torch._C._cuda_getDevice() == index:
+        return fn(*fn_args)
+    with torch.cuda.device(index):
+        return fn(*fn_args)
+
+
 def build_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor | None, *, block_n: int = 64,
                num_splits: int | None = None, sm_scale: float | None = None, kernel: str = "auto",
                result_f32: torch.Tensor | None = None, result_lse: torch.Tensor | None = None,

@@ -14,7 +14,7 @@ import typing
 import torch
 
 from . import _cabi
-from .decode import _call_on_device
+from .decode import _call_on_index, _current_stream
 
 MAX_BATCH = 8192
 
@@ -31,13 +31,14 @@ class StepPlan(typing.NamedTuple):
     num_free: torch.Tensor  # [1] int32
 
 
-def _vector(t: torch.Tensor, what: str, dtype: torch.dtype, size: int | None, device: torch.device) -> int:
-    if t.dtype != dtype or t.dim() != 1 or (size is not None and t.shape[0] != size):
-        raise ValueError(f"{what} must be a vector of {dtype}" + ("" if size is None else f" with {size} entries"))
-    if t.device != device:
-        raise ValueError(f"{what} must be on {device}")
-    if t.shape[0] > 1 and t.stride(0) != 1:
-        raise ValueError(f"{what} must be contiguous")
+def _vector(t: torch.Tensor, what: str, dtype: torch.dtype, size: int | None, index: int) -> int:
+    """Address of a checked vector; cheap where all is well (a plan is microseconds of work)."""
+    if (t.dtype is not dtype or t.dim() != 1 or t.get_device() != index or not t.is_contiguous()
+            or (size is not None and t.numel() != size)):
+        if t.get_device() != index:
+            raise ValueError(f"{what} must be on the block table's device")
+        raise ValueError(f"{what} must be a contiguous vector of {dtype}"
+                         + ("" if size is None else f" with {size} entries"))
     return t.data_ptr()
 
 
@@ -65,47 +66,51 @@ def plan_step(block_table: torch.Tensor, context_lens: torch.Tensor, new_tokens:
     """
     if not block_table.is_cuda:
         raise _cabi.NativeLibraryError("plan_step runs on CUDA tensors only; there is no CPU path")
-    dev = block_table.device
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be int32 [batch, max_blocks]")
     b, width = block_table.shape
-    if width > 1 and block_table.stride(1) != 1:
+    stride, inner = block_table.stride()
+    if width < 1:
+        raise ValueError("block_table must be int32 [batch, max_blocks]")
+    if inner != 1 and width > 1:
         raise ValueError("block_table rows must be contiguous")
-    if b > 1 and block_table.stride(0) < width:
-        raise ValueError("block_table rows must not overlap")
-    num_tokens = int(num_tokens)
-    if num_tokens < 0 or int(block_size) <= 0:
+    if stride < width:
+        if b > 1:
+            raise ValueError("block_table rows must not overlap")
+        stride = width
+    if num_tokens < 0 or block_size <= 0:
         raise ValueError("num_tokens must not be negative and block_size must be positive")
     if b > MAX_BATCH:
         raise ValueError(f"at most {MAX_BATCH} requests")
-    ctx = _vector(context_lens, "context_lens", torch.int32, b, dev)
-    new = _vector(new_tokens, "new_tokens", torch.int32, b, dev)
-    free = _vector(free_blocks, "free_blocks", torch.int32, None, dev)
-    nfree = _vector(num_free, "num_free", torch.int32, 1, dev)
+    index = block_table.get_device()
+    i32 = torch.int32
+    ctx = _vector(context_lens, "context_lens", i32, b, index)
+    new = _vector(new_tokens, "new_tokens", i32, b, index)
+    free = _vector(free_blocks, "free_blocks", i32, None, index)
+    nfree = _vector(num_free, "num_free", i32, 1, index)
     if out is None:
+        dev = block_table.device
         slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
         positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-        narrow = torch.empty(2 * b + 2, dtype=torch.int32, device=dev)
-        starts, lens, left = narrow.split((b + 1, b, 1))
+        starts, lens, left = torch.empty(2 * b + 2, dtype=i32, device=dev).split((b + 1, b, 1))
         out = StepPlan(slots, positions, starts, lens, left)
-        at = narrow.data_ptr()
+        at = starts.data_ptr()
         ptrs = (slots.data_ptr(), positions.data_ptr(), at, at + 4 * (b + 1), at + 4 * (2 * b + 1))
     else:
-        ptrs = (_vector(out.slot_mapping, "out.slot_mapping", torch.int64, num_tokens, dev),
-                _vector(out.positions, "out.positions", torch.int64, num_tokens, dev),
-                _vector(out.query_start_loc, "out.query_start_loc", torch.int32, b + 1, dev),
-                _vector(out.seq_lens, "out.seq_lens", torch.int32, b, dev),
-                _vector(out.num_free, "out.num_free", torch.int32, 1, dev))
+        ptrs = (_vector(out.slot_mapping, "out.slot_mapping", torch.int64, num_tokens, index),
+                _vector(out.positions, "out.positions", torch.int64, num_tokens, index),
+                _vector(out.query_start_loc, "out.query_start_loc", i32, b + 1, index),
+                _vector(out.seq_lens, "out.seq_lens", i32, b, index),
+                _vector(out.num_free, "out.num_free", i32, 1, index))
         _refuse_overlap(block_table, context_lens, new_tokens, free_blocks, num_free, out)
     word = 0
     if status is not None:
-        if status.dtype != torch.int32 or status.numel() < 1 or status.device != dev:
+        if status.dtype is not i32 or status.numel() < 1 or status.get_device() != index:
             raise ValueError("status must be an int32 tensor on the same device")
         word = status.data_ptr()
-    block = _PACK.pack(block_table.data_ptr(), max(block_table.stride(0), width), ctx, new, free, nfree, *ptrs, b, width,
-                       int(block_size), free_blocks.shape[0], num_tokens, word,
-                       torch.cuda.current_stream(dev).cuda_stream)
-    rc = _call_on_device(dev, _cabi.load().pd_plan_step, block)
+    block = _PACK.pack(block_table.data_ptr(), stride, ctx, new, free, nfree, *ptrs, b, width, block_size,
+                       free_blocks.numel(), num_tokens, word, _current_stream(index))
+    rc = _call_on_index(index, _cabi.load().pd_plan_step, block)
     if rc != 0:
         _cabi.check(rc, "pd_plan_step")
     return out

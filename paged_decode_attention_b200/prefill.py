@@ -7,25 +7,26 @@
 
 They read the cache that ``paged_decode`` reads, after ``cache_write`` has stored the new tokens.
 ``kernel="auto"`` takes the kernels on the matrix units where they serve the request (head_dim 64
-and 128, pages of a multiple of 16 tokens up to 256, q of the cache's own 16-bit type or fp16 with
-8-bit pages, 16-byte aligned rows) and a general kernel on the CUDA cores everywhere else.  There
+and 128, q of the cache's own 16-bit type or fp16 with 8-bit pages, 16-byte aligned rows; single tokens:
+pages of a multiple of 16 tokens up to 256, groups of up to 16 heads) and a general kernel on the CUDA cores everywhere else.  There
 is no CPU or PyTorch fallback.
 """
 
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _cabi
 from .cache import PagedKVCache
-from .config import KV_CODE
-from .decode import _call_on_device
+from .config import KV_CODE, torch_dtype
+from .decode import _call_on_index, _current_stream
 
 _PACK = _cabi.packer(_cabi.PdPrefillArgs)
 _INDEX = {name: i for i, (name, _) in enumerate(_cabi.PdPrefillArgs._fields_)}
-_WORKSPACE, _WORKSPACE_BYTES = _INDEX["workspace"], _INDEX["workspace_bytes"]
+_SCRATCH, _SCRATCH_AT = struct.Struct("@PQ"), _cabi.PdPrefillArgs.workspace.offset
 
 
 def build_prefill_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, query_start_loc: torch.Tensor | None, *,
@@ -34,43 +35,48 @@ def build_prefill_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, 
                        max_seq_len: int = 0, status: torch.Tensor | None = None, sm_count: int = 0,
                        stream: int = 0) -> list:
     """The checked values of a ``PdPrefillArgs`` block, in its field order, without scratch."""
-    k, v, bt, sl = cache.k_cache, cache.v_cache, cache.block_table, cache.seq_lens
-    dev = k.device
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+    k, v, bt, sl, shape = cache.k_cache, cache.v_cache, cache.block_table, cache.seq_lens, cache.shape
+    dev = k.get_device()
+    k_stride = k.stride()
+    if k.dim() != 4 or k.shape != v.shape or k_stride != v.stride() or k.dtype is not v.dtype or k_stride[3] != 1:
         raise ValueError("k_cache and v_cache must be alike [num_blocks, block_size, H_kv, D] with head_dim contiguous")
+    if k.dtype is not torch_dtype(cache.kv_dtype):
+        raise ValueError(f"cache tensors are {k.dtype}, kv_dtype says {cache.kv_dtype}")
     num_blocks, page, hkv, d = k.shape
-    hq = cache.shape.num_q_heads
-    if hkv != cache.shape.num_kv_heads or page != cache.block_size or d != cache.shape.head_dim:
+    hq = shape.num_q_heads
+    if hkv != shape.num_kv_heads or page != cache.block_size or d != shape.head_dim:
         raise ValueError("cache tensors disagree with cache.shape / cache.block_size")
     if hq % maps or hkv % maps or hq % hkv:
         raise ValueError(f"{hq} query heads and {hkv} kv heads do not form whole groups" + (" of pairs" if maps == 2 else ""))
-    if maps == 1:
-        if q.dim() != 3 or q.shape[1] != hq or q.shape[2] != d:
-            raise ValueError(f"q must be [rows, {hq}, {d}]")
-        map_stride = 0
-    else:
-        if q.dim() != 4 or q.shape[1] != hq // 2 or q.shape[2] != 2 or q.shape[3] != d:
-            raise ValueError(f"q must be [rows, {hq // 2}, 2, {d}]")
-        map_stride = q.stride(2)
-    if q.dtype not in _cabi.IO_CODE:
+    q_shape, q_stride = q.shape, q.stride()
+    rows = q_shape[0] if q_shape else 0
+    want = (rows, hq, d) if maps == 1 else (rows, hq // 2, 2, d)
+    if q_shape != want:
+        raise ValueError(f"q must be [rows, {', '.join(map(str, want[1:]))}]")
+    map_stride = q_stride[2] if maps == 2 else 0
+    io = _cabi.IO_CODE.get(q.dtype)
+    if io is None:
         raise ValueError(f"q dtype {q.dtype} not supported (fp16 or bf16)")
-    if q.stride(-1) != 1:
+    if q_stride[-1] != 1:
         raise ValueError("head_dim must be contiguous in q")
-    rows = q.shape[0]
-    if tuple(out.shape) != (rows, hq // maps, maps * d) or out.dtype != q.dtype or out.stride(2) != 1:
+    out_stride = out.stride()
+    if out.shape != (rows, hq // maps, maps * d) or out.dtype is not q.dtype or out_stride[2] != 1:
         raise ValueError(f"out must be {q.dtype} [{rows}, {hq // maps}, {maps * d}] with the last dimension contiguous")
-    if bt.dtype != torch.int32 or sl.dtype != torch.int32 or bt.dim() != 2 or sl.dim() != 1:
+    if bt.dtype is not torch.int32 or sl.dtype is not torch.int32 or bt.dim() != 2 or sl.dim() != 1:
         raise ValueError("block_table [B, max_blocks] and seq_lens [B] must be int32")
-    if (bt.shape[1] > 1 and bt.stride(1) != 1) or not sl.is_contiguous():
-        raise ValueError("block_table rows and seq_lens must be contiguous")
     b, width = bt.shape
-    if sl.shape[0] != b:
+    bt_stride, inner = bt.stride()
+    if (width > 1 and inner != 1) or not sl.is_contiguous():
+        raise ValueError("block_table rows and seq_lens must be contiguous")
+    if b > 1 and bt_stride < width:
+        raise ValueError("block_table rows must not overlap")
+    if sl.numel() != b:
         raise ValueError(f"seq_lens has {sl.shape[0]} entries for {b} block_table rows")
     tensors = [q, out, v, bt, sl]
     starts = 0
     if query_start_loc is not None:
-        if query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1 or query_start_loc.shape[0] != b + 1 \
-                or not query_start_loc.is_contiguous():
+        if query_start_loc.dtype is not torch.int32 or query_start_loc.dim() != 1 \
+                or query_start_loc.numel() != b + 1 or not query_start_loc.is_contiguous():
             raise ValueError(f"query_start_loc must be a contiguous int32 vector of {b + 1} entries")
         starts = query_start_loc.data_ptr()
         tensors.append(query_start_loc)
@@ -81,25 +87,29 @@ def build_prefill_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, 
     if (ks is None) != (vs is None):
         raise ValueError("k_scale and v_scale must both be given or both be None")
     if ks is not None:
-        if ks.dtype != torch.float16 or vs.dtype != torch.float16 or tuple(ks.shape) != (num_blocks, page, hkv) \
-                or ks.shape != vs.shape or ks.stride() != vs.stride() or (hkv > 1 and ks.stride(2) != 1):
+        s_stride = ks.stride()
+        if ks.dtype is not torch.float16 or vs.dtype is not torch.float16 or ks.shape != (num_blocks, page, hkv) \
+                or ks.shape != vs.shape or s_stride != vs.stride() or (hkv > 1 and s_stride[2] != 1):
             raise ValueError("scales must be fp16 [num_blocks, block_size, H_kv], alike, with the head index contiguous")
-        scales = (ks.data_ptr(), vs.data_ptr(), ks.stride(0), ks.stride(1))
+        scales = (ks.data_ptr(), vs.data_ptr(), s_stride[0], s_stride[1])
         tensors += (ks, vs)
     lam_ptr, lam_t, lam_h, lam_value, weight = 0, 0, 0, 0.0, 0
     if maps == 2:
         if isinstance(lam, torch.Tensor):
             if lam.dtype != torch.float32 or lam.dim() > 2:
                 raise ValueError("lam must be fp32: one value, [pairs] or [rows, pairs]")
-            lam = lam.expand(rows, hq // 2)  # raises when the shape does not broadcast
-            lam_ptr, lam_t, lam_h = lam.data_ptr(), lam.stride(0), lam.stride(1)
+            if lam.dim() == 1 and lam.numel() == hq // 2:  # the usual form, one value a pair
+                lam_ptr, lam_t, lam_h = lam.data_ptr(), 0, lam.stride(0)
+            else:
+                wide = lam.expand(rows, hq // 2)  # raises when the shape does not broadcast
+                lam_ptr, lam_t, lam_h = wide.data_ptr(), wide.stride(0), wide.stride(1)
             tensors.append(lam)
         else:
             lam_value = float(lam)
         if norm_weight is not None:
             if not norm:
                 raise ValueError("norm_weight without norm")
-            if norm_weight.dtype != torch.float32 or tuple(norm_weight.shape) != (2 * d,) or not norm_weight.is_contiguous():
+            if norm_weight.dtype is not torch.float32 or norm_weight.shape != (2 * d,) or not norm_weight.is_contiguous():
                 raise ValueError(f"norm_weight must be a contiguous fp32 vector of {2 * d} entries")
             weight = norm_weight.data_ptr()
             tensors.append(norm_weight)
@@ -110,15 +120,15 @@ def build_prefill_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, 
         word = status.data_ptr()
         tensors.append(status)
     for t in tensors:
-        if t.device != dev:
-            raise ValueError(f"all tensors must be on {dev}, one is on {t.device}")
+        if t.get_device() != dev:
+            raise ValueError("all tensors must be on the cache's device")
     if kernel not in _cabi.KERNEL_CODE:
         raise ValueError(f"kernel must be one of {sorted(_cabi.KERNEL_CODE)}")
-    return [q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), map_stride, out.stride(0), out.stride(1),
-            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), *scales,
-            bt.data_ptr(), max(bt.stride(0), width), sl.data_ptr(), starts,
-            rows, b, hq, hkv, d, page, num_blocks, width, KV_CODE[cache.kv_dtype], _cabi.IO_CODE[q.dtype],
-            cache.shape.softmax_scale if sm_scale is None else float(sm_scale), maps,
+    return [q.data_ptr(), out.data_ptr(), q_stride[0], q_stride[1], map_stride, out_stride[0], out_stride[1],
+            k.data_ptr(), v.data_ptr(), k_stride[0], k_stride[1], k_stride[2], *scales,
+            bt.data_ptr(), max(bt_stride, width), sl.data_ptr(), starts,
+            rows, b, hq, hkv, d, page, num_blocks, width, KV_CODE[cache.kv_dtype], io,
+            shape.softmax_scale if sm_scale is None else float(sm_scale), maps,
             lam_ptr, lam_t, lam_h, lam_value, weight, float(eps), float(out_scale), int(bool(norm)),
             _cabi.KERNEL_CODE[kernel], int(sm_count), int(max_seq_len), 0, 0, word, stream]
 
@@ -135,27 +145,24 @@ def _run(entry: str, q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor | N
          query_start_loc: torch.Tensor | None, maps: int, **kw) -> torch.Tensor:
     if not q.is_cuda:
         raise _cabi.NativeLibraryError(f"{entry} runs on CUDA tensors only; there is no CPU path")
-    dev = q.device
+    index = q.get_device()
     if out is None:
-        shape = (q.shape[0], q.shape[1], maps * q.shape[-1])
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-    values = build_prefill_args(q, cache, out, query_start_loc, maps=maps,
-                                stream=torch.cuda.current_stream(dev).cuda_stream, **kw)
+        out = torch.empty((q.shape[0], q.shape[1], maps * q.shape[-1]), dtype=q.dtype, device=q.device)
+    values = build_prefill_args(q, cache, out, query_start_loc, maps=maps, stream=_current_stream(index), **kw)
     if q.shape[0] == 0 or cache.batch == 0:
         return out
     lib = _cabi.load()
     need = ctypes.c_uint64(0)
     block = _PACK.pack(*values)
-    rc = _call_on_device(dev, lib.pd_prefill_workspace_bytes, block, ctypes.byref(need))
+    rc = _call_on_index(index, lib.pd_prefill_workspace_bytes, block, ctypes.byref(need))
     if rc != 0:
         _cabi.check(rc, "pd_prefill_workspace_bytes")
     if need.value:
         # Scratch of this call alone, from torch's allocator: ordered by the stream, and inside a
         # capture a part of that graph, so no two graphs or streams share it.
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        values[_WORKSPACE], values[_WORKSPACE_BYTES] = ws.data_ptr(), need.value
-        block = _PACK.pack(*values)
-    rc = _call_on_device(dev, getattr(lib, entry), block)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        block = block[:_SCRATCH_AT] + _SCRATCH.pack(ws.data_ptr(), need.value) + block[_SCRATCH_AT + _SCRATCH.size:]
+    rc = _call_on_index(index, getattr(lib, entry), block)
     if rc != 0:
         _cabi.check(rc, entry)
     return out
