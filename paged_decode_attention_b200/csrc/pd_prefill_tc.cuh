@@ -46,6 +46,7 @@
 namespace pd {
 
 constexpr int kTcBlock = 128;      // keys of one block, rows of one tile
+constexpr int kTcLeast = 4;        // key blocks a split has at least: what its start and end cost is about that
 constexpr int kTcMetaRing = 16;    // blocks whose bad-page masks are kept
 constexpr int kTcSmem = 227 * 1024;
 
@@ -164,6 +165,38 @@ __host__ __device__ constexpr uint32_t tc_idesc(bool bf16, int n, bool b_mn) {
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// A bounded wait for a barrier phase, by every lane of a warp; the answer is the warp's.  try_wait suspends
+// the warp for up to kTcSuspendNs at a time, so a waiting warp costs the others next to nothing; after
+// kTcTries of them (50 ms at the very least) it gives up, raises the CTA's abort flag and PD_DEV_TIMEOUT.
+// Inline on purpose: a call keeps the softmax's 128 scores from staying in registers.
+constexpr int kTcTries = 1 << 22;
+constexpr unsigned kTcSuspendNs = 1000;
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, uint32_t* status, volatile int* abort_flag) {
+  bool ok = false;
+  for (int i = 0; i < kTcTries; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(kTcSuspendNs)
+        : "memory");
+    ok = done != 0;
+    if (ok || *abort_flag) break;
+  }
+  if (__all_sync(0xffffffffu, ok)) return true;
+  *abort_flag = 1;
+  if (status) atomicOr(status, PD_DEV_TIMEOUT);
+  return false;
+}
+
+// Gives what is still in flight a bounded chance to end (the abort flag is up).
+__device__ __forceinline__ void tc_drain(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < kTcTries && !mbar_try_wait(bar, parity); ++i) {
+  }
+}
+
 // Two floats in one instruction, and the largest of three.
 __device__ __forceinline__ void tc_fma2(float& x, float& y, float f, float g) {  // (x, y) = (x, y) * f + g
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
@@ -235,6 +268,50 @@ __device__ __forceinline__ void tc_copy_pages(uint32_t dst, const __half* cache,
       cp_async16(to[i % (8 / RPI)] + (2 * g + i / (8 / RPI)) * 1024, src, i * RPI < rows);
       src += step;
     }
+  }
+}
+
+// Offset of a token of the request in a cache tensor (kv head 0), and in the scales, or -1: no such key, or
+// one in no page of the pool, which is noted in its block's mask.
+__device__ __forceinline__ int64_t tc_place(const Params& p, int request, int token, int kv_end, unsigned* mask, unsigned bits,
+                                            int64_t& scale_at) {
+  scale_at = 0;
+  if (token >= kv_end) return -1;
+  const int page = token / p.page;
+  const int id = __ldg(p.block_table + (int64_t)request * p.bt_stride + page);
+  if ((unsigned)id < (unsigned)p.num_blocks) {
+    scale_at = scale_offset(p, id, token - page * p.page, 0);
+    return kv_row_offset(p, id, token - page * p.page, 0);
+  }
+  if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
+  atomicOr(mask, bits);
+  return -1;
+}
+
+// The 16-byte pieces of an 8-bit tile that thread `me` of 128 takes: piece c of the rows r0, r0 + 128 / P, ..
+// `where` of lane l: tc_place of token 16 l of the block (whole pages of 16 tokens).
+template <int P, int D, int PM>
+__device__ __forceinline__ void tc_fetch(const Params& p, int request, int j, int h, const void* cache, bool whole, int64_t where,
+                                         int kv_end, unsigned* mask, int me, uint4 (&x)[PM]) {
+  const int c = me % P, r0 = me / P;
+  const char* mine = (const char*)cache + (int64_t)(h + c * 16 / D) * p.kv_sh + c * 16 % D;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int r = r0 + i * (128 / P);
+    int64_t at;
+    bool live;
+    if (whole) {
+      at = __shfl_sync(0xffffffffu, where, r / 16);
+      live = at >= 0 && j * kTcBlock + r < kv_end;
+      at += (int64_t)(r & 15) * p.kv_st;
+    } else {
+      int64_t unused;
+      at = tc_place(p, request, j * kTcBlock + r, kv_end, mask + r / 32, 1u << (r & 31), unused);
+      live = at >= 0;
+    }
+    // always a load, of some row of the pool where there is none: loads behind branches went one by one
+    const uint4 y = __ldg(reinterpret_cast<const uint4*>(mine + (live ? at : 0)));
+    x[i] = live ? y : make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -383,7 +460,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   int rows_of[2], begin[2], end[2];  // rows, first and last + 1 key block
   const int last_row = tile.row0 + tile.count - 1;
   const int blocks = (tc_limit(tile, last_row, p.group) + kTcBlock - 1) / kTcBlock;  // of the longest row
-  const int chunk = (blocks + tp.splits - 1) / tp.splits;
+  const int chunk = tp.splits > 1 ? max((blocks + tp.splits - 1) / tp.splits, kTcLeast) : blocks;
   const int j0 = min(split * chunk, blocks), j1 = min(j0 + chunk, blocks);
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -445,7 +522,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / each)) & 1u) << e;
           }
         }
-        if (!__all_sync(kFull, mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag))) break;
+        if (!tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag)) break;
         if (k == 0 && lane == 0)  // ahead of the block's scores
           *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
         if (by_tma) {
@@ -469,7 +546,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           __syncwarp();
           if (tail) {
             tail_used = true;
-            if (!__all_sync(kFull, mbar_wait(tail_bar, 0, p.status, abort_flag))) break;  // the one tail of this CTA
+            if (!tc_wait(tail_bar, 0, p.status, abort_flag)) break;  // the one tail of this CTA
             const int to = (live / bt + 1) * bt;
             for (int i = lane; i < (to - live) * C::VC * 8; i += 32) {
               const int r = live + i / 8 % (to - live), c = i / 8 / (to - live);
@@ -496,9 +573,9 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           int j, k;
           tc_unit<C::KT>(u, j0, j, k);
           if ((k < 0) == (warp == 8))
-            mbar_wait_slow(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u, nullptr, abort_flag, false);
+            tc_drain(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u);
         }
-        if (tail_used) mbar_wait_slow(tail_bar, 0, nullptr, abort_flag, false);
+        if (tail_used) tc_drain(tail_bar, 0);
       }
     }
   }
@@ -514,86 +591,68 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       const int nb = jend - j0;
       const int units = nb > 0 ? nb * (C::KT + 1) : 0;
       const bool whole = p.page % 16 == 0;               // 16 tokens lie in one page
-      // lane l < 8: block id of tokens 16 l .. of block j (-1: none), and whether there should have been one
-      auto fetch_ids = [&](int j) {
-        const int token = j * kTcBlock + 16 * lane;
-        int id = -1;
-        if (whole && lane < 8 && token < kv_end) id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + token / p.page);
-        return id;
+      // lane l < 8 for tokens 16 l .. of block j
+      auto locate = [&](int j, int64_t& scale_at) -> int64_t {
+        scale_at = 0;
+        if (!whole || lane >= 8) return -1;
+        return tc_place(p, tile.request, j * kTcBlock + 16 * lane, kv_end, meta + 4 * (j & (kTcMetaRing - 1)) + lane / 2,
+                        0xffffu << (16 * (lane & 1)), scale_at);
       };
-      // offset of token r of block j in a cache tensor of kv head h, -1: no such key
-      auto place = [&](int ids, int j, int r, int& off) {
-        const int token = j * kTcBlock + r;
-        const int from = __shfl_sync(kFull, ids, r / 16);
-        off = 0;
-        if (token >= kv_end) return -1;
-        const int page = token / p.page;
-        const int id = whole ? from : __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
-        off = token - page * p.page;
-        if ((unsigned)id < (unsigned)p.num_blocks) return id;
-        if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
-        atomicOr(&meta[4 * (j & (kTcMetaRing - 1)) + r / 32], 1u << (r & 31));
-        return -1;
-      };
-      auto fetch = [&](int j, int k, int ids, uint4 (&x)[PM], float (&sc)[SCALED ? C::KT + C::VH : 1]) {
-        const int pieces = k < 0 ? PV : PK;
-#pragma unroll
-        for (int i = 0; i < PM; ++i) {
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (i >= pieces) continue;
-          const int n = me + i * 128, r = n / pieces, c = n % pieces;
-          int off;
-          const int id = place(ids, j, r, off);
-          if (id >= 0) {
-            const int col = k < 0 ? slice * C::DV + c * 16 : c * 16;
-            const int64_t at = kv_row_offset(p, id, off, head * MAPS + (k < 0 ? col / D : k)) + col % D;
-            x[i] = __ldg(reinterpret_cast<const uint4*>((const char*)(k < 0 ? p.v : p.k) + at));
-          }
-        }
+      auto fetch_unit = [&](int j, int k, int64_t where, int64_t scale_where, uint4 (&x)[PM], __half (&sc)[SCALED ? C::KT + C::VH : 1]) {
+        unsigned* mask = meta + 4 * (j & (kTcMetaRing - 1));
+        if (k < 0) tc_fetch<PV, D, PM>(p, tile.request, j, head * MAPS + slice * C::DV / D, p.v, whole, where, kv_end, mask, me, x);
+        else tc_fetch<PK, D, PM>(p, tile.request, j, head * MAPS + k, p.k, whole, where, kv_end, mask, me, x);
         if constexpr (SCALED) {
           // the block's scales, K's and V's, with its first K tile: the softmax needs them ahead of V itself
           if (k == 0) {
-            int off;
-            const int id = place(ids, j, me, off);
+            int64_t at = __shfl_sync(kFull, scale_where, me / 16);
+            bool live = __shfl_sync(kFull, where, me / 16) >= 0 && j * kTcBlock + me < kv_end;
+            at += (int64_t)(me & 15) * p.sc_st;
+            if (!whole) live = tc_place(p, tile.request, j * kTcBlock + me, kv_end, mask + me / 32, 1u << (me & 31), at) >= 0;
+            at = (live ? at : 0) + head * MAPS;
 #pragma unroll
-            for (int z = 0; z < C::KT + C::VH; ++z) sc[z] = 0.f;
-            if (id >= 0) {
-              const int64_t at = scale_offset(p, id, off, head * MAPS);
+            for (int z = 0; z < C::KT; ++z) {
+              const __half y = __ldg(p.k_scale + at + z);
+              sc[z] = live ? y : __ushort_as_half(0);
+            }
 #pragma unroll
-              for (int z = 0; z < C::KT; ++z) sc[z] = __half2float(__ldg(p.k_scale + at + z));
-#pragma unroll
-              for (int z = 0; z < C::VH; ++z)
-                sc[C::KT + z] = kBoost * __half2float(__ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0)));
+            for (int z = 0; z < C::VH; ++z) {
+              const __half y = __ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0));
+              sc[C::KT + z] = live ? y : __ushort_as_half(0);
             }
           }
         }
       };
-      int ids = fetch_ids(j0), ids_next = fetch_ids(j0 + 1);  // of block idj and the one behind it
+      // where the tokens of block idj and of the one behind it lie
+      int64_t s_here, s_next;
+      int64_t here = locate(j0, s_here), next = locate(j0 + 1, s_next);
       int idj = j0;
       uint4 x[PM];
-      float sc[SCALED ? C::KT + C::VH : 1];
-      if (units > 0) fetch(j0, 0, ids, x, sc);
+      __half sc[SCALED ? C::KT + C::VH : 1];
+      if (units > 0) fetch_unit(j0, 0, here, s_here, x, sc);
       bool ok = true;
       for (int unit = 0; unit < units && ok; ++unit) {
         int j, k;
         tc_unit<C::KT>(unit, j0, j, k);
         uint4 nx[PM];
-        float nsc[SCALED ? C::KT + C::VH : 1];
+        __half nsc[SCALED ? C::KT + C::VH : 1];
         if (unit + 1 < units) {
           int j2, k2;
           tc_unit<C::KT>(unit + 1, j0, j2, k2);
-          if (k2 == 0 && me < 4) meta[4 * ((j2 + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;  // read long ago, written far ahead
-          // a block's V comes behind its K, the next block's K behind that: its ids are fetched with this V
+          // a block's V comes behind its K, the next block's K behind that: its tokens are located with this V
           if (j2 > idj && k2 < 0) {
-            ids = ids_next;
+            here = next;
+            s_here = s_next;
             ++idj;
-            ids_next = fetch_ids(idj + 1);
+            // the mask of a block read long ago, of one to be located far ahead
+            if (me < 4) meta[4 * ((idj + 1 + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;
+            next = locate(idj + 1, s_next);
           }
-          fetch(j2, k2, j2 > idj ? ids_next : ids, nx, nsc);
+          fetch_unit(j2, k2, j2 > idj ? next : here, j2 > idj ? s_next : s_here, nx, nsc);
         }
         const int st = unit % C::NSLOT;
         const uint32_t dst = ring0 + st * C::SLOT;
-        ok = __all_sync(kFull, mbar_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag));
+        ok = tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag);
         if (!ok) break;
         const int pieces = k < 0 ? PV : PK;
 #pragma unroll
@@ -623,7 +682,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           if (k == 0) {
 #pragma unroll
             for (int z = 0; z < C::KT + C::VH; ++z)
-              scales[(j % C::SCALE_RING) * C::SCALE_FLOATS + z * 128 + me] = sc[z];
+              scales[(j % C::SCALE_RING) * C::SCALE_FLOATS + z * 128 + me] = __half2float(sc[z]) * (z < C::KT ? 1.f : kBoost);
           }
         }
         fence_proxy_async();
@@ -644,9 +703,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     uint32_t mine;
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(mine));
     bool ok = true;
-    // every lane waits (the outcome is the warp's: all see the same phase or the same abort flag)
     auto wait_bar = [&](uint32_t bar, uint32_t parity) {
-      return __all_sync(kFull, mbar_wait(bar, parity, p.status, abort_flag)) != 0;
+      return tc_wait(bar, parity, p.status, abort_flag);
     };
     auto scores = [&](int t, int kslot) {  // S_t = Q_t K^T
       const uint64_t qd = tc_desc(q0 + t * C::QTILE, 1024, 0), kd = tc_desc(ring0 + kslot * C::SLOT, 1024, 0);
@@ -750,7 +808,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       }
       if (!ok) {  // products in flight get a bounded chance to end before tensor memory is freed
         tc_commit(drain_bar, mine);
-        mbar_wait_slow(drain_bar, 0, nullptr, abort_flag, false);
+        tc_drain(drain_bar, 0);
       }
     }
     __syncwarp();
@@ -793,7 +851,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = j0; j < end[t]; ++j) {
-      ok = mbar_wait(s_full + 8 * t, (uint32_t)(j - j0) & 1u, p.status, abort_flag);
+      ok = tc_wait(s_full + 8 * t, (uint32_t)(j - j0) & 1u, p.status, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const volatile unsigned* bad = meta + 4 * (j & (kTcMetaRing - 1));
@@ -904,7 +962,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
 
     // ---- results ----------------------------------------------------------------------------------------
     // (maps = 2: both tiles' products, of which the second tile's are the last: the ring is written below)
-    if (ok && end[t] > j0) ok = mbar_wait(o_done + 8 * (MAPS == 2 ? 1 : t), 0, p.status, abort_flag);
+    if (ok && end[t] > j0) ok = tc_wait(o_done + 8 * (MAPS == 2 ? 1 : t), 0, p.status, abort_flag);
     tc_fence_after();
     const bool any = end[t] > j0;  // else tensor memory holds nothing of this tile
     const float inv = l > 0.f || l != l ? 1.f / (l * kBoost) : 0.f;
@@ -922,12 +980,10 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           tc_ld32(o_at + c0, o);
           tc_wait_ld();
         }
-        if (live && ok) {
+        if (live && ok && any && inv != 0.f) {  // a row without keys is told by its log-sum-exp
           float4* dst = reinterpret_cast<float4*>(tp.part_o + at * (MAPS * D) + slice * C::DV + c0);
 #pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            dst[c / 4] = any && inv != 0.f ? make_float4(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv)
-                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = 0; c < 32; c += 4) dst[c / 4] = make_float4(o[c] * inv, o[c + 1] * inv, o[c + 2] * inv, o[c + 3] * inv);
         }
       }
       if (live && ok && slice == 0) tp.part_lse[at] = l > 0.f || l != l ? m + log2f(l) : -INFINITY;
