@@ -70,7 +70,12 @@ struct TcCfg {
   static constexpr int FIT = (kTcSmem - FIXED) / SLOT;
   static constexpr int NSLOT = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = FIXED + NSLOT * SLOT;
-  static constexpr int WARPS = WIDEN ? 14 : 12;            // softmax 0-3 and 4-7, matrix units 9, loaders 8, 10, 11 (or widening 10-13)
+  // softmax 0-3 and 4-7, matrix units 9, loaders 8, 10, 11; widening 12-15
+  static constexpr int WARPS = WIDEN ? 16 : 12;
+  // Registers.  A scheduler has a warp of each tile's softmax, one of the third group and, with 8-bit pages,
+  // one that widens; what they hold adds up to the launch's 3 * 168 or 4 * 128.
+  static constexpr int REGS_SOFTMAX = WIDEN ? 176 : 200, REGS_THIRD = WIDEN ? 56 : 104, REGS_WIDEN = 104;
+  static_assert(WIDEN ? 2 * REGS_SOFTMAX + REGS_THIRD + REGS_WIDEN <= 4 * 128 : 2 * REGS_SOFTMAX + REGS_THIRD <= 3 * 168, "registers");
   static constexpr int THREADS = WARPS * 32;
   static_assert(NSLOT >= 3 && SMEM <= kTcSmem, "shared memory");
 };
@@ -289,30 +294,33 @@ __device__ __forceinline__ int64_t tc_place(const Params& p, int request, int to
 }
 
 // The 16-byte pieces of an 8-bit tile that thread `me` of 128 takes: piece c of the rows r0, r0 + 128 / P, ..
-// `where` of lane l: tc_place of token 16 l of the block (whole pages of 16 tokens).
+// `where` of lane l: tc_place of token 16 l of the block (whole pages of 16 tokens).  Bit i of the answer:
+// piece i exists.  All addresses first, then all loads, and nothing that uses one: the loads are to be in
+// flight together, until the pieces are widened (a use behind each load made a tile cost eight round trips).
 template <int P, int D, int PM>
-__device__ __forceinline__ void tc_fetch(const Params& p, int request, int j, int h, const void* cache, bool whole, int64_t where,
-                                         int kv_end, unsigned* mask, int me, uint4 (&x)[PM]) {
+__device__ __forceinline__ unsigned tc_fetch(const Params& p, int request, int j, int h, const void* cache, bool whole, int64_t where,
+                                             int kv_end, unsigned* mask, int me, uint4 (&x)[PM]) {
   const int c = me % P, r0 = me / P;
   const char* mine = (const char*)cache + (int64_t)(h + c * 16 / D) * p.kv_sh + c * 16 % D;
+  const uint4* from[P];
+  unsigned live = 0;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int r = r0 + i * (128 / P);
     int64_t at;
-    bool live;
     if (whole) {
       at = __shfl_sync(0xffffffffu, where, r / 16);
-      live = at >= 0 && j * kTcBlock + r < kv_end;
-      at += (int64_t)(r & 15) * p.kv_st;
+      if (at >= 0) at = j * kTcBlock + r < kv_end ? at + (int64_t)(r & 15) * p.kv_st : -1;
     } else {
       int64_t unused;
       at = tc_place(p, request, j * kTcBlock + r, kv_end, mask + r / 32, 1u << (r & 31), unused);
-      live = at >= 0;
     }
-    // always a load, of some row of the pool where there is none: loads behind branches went one by one
-    const uint4 y = __ldg(reinterpret_cast<const uint4*>(mine + (live ? at : 0)));
-    x[i] = live ? y : make_uint4(0, 0, 0, 0);
+    live |= (at >= 0 ? 1u : 0u) << i;
+    from[i] = reinterpret_cast<const uint4*>(mine + (at >= 0 ? at : 0));  // some row of the pool where there is none
   }
+#pragma unroll
+  for (int i = 0; i < P; ++i) x[i] = __ldg(from[i]);
+  return live;
 }
 
 // What a CTA works on.
@@ -472,120 +480,14 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   const int jend = max(end[0], end[1]);
   const int kv_end = tc_limit(tile, last_row, p.group);  // keys from here on are zeros in shared memory
 
-  // ================================ loaders (16-bit pages) =============================================
-  // V's tiles: warp 8; K's: warps 10 and 11 in turn.
-  if (warp == 8 || (!C::WIDEN && warp >= 10)) {
-    if constexpr (!C::WIDEN) {
-      const int nb = jend - j0;
-      const int units = nb > 0 ? nb * (C::KT + 1) : 0;
-      const bool whole = p.page % 16 == 0;                 // 16 tokens lie in one page
-      const bool by_tma = whole && (warp == 8 || p.page % 64 == 0);
-      const int bt = tp.box_tokens, boxes = kTcBlock / bt;
-      int turn = 0, issued = -1;
-      bool tail_used = false;
-      for (int unit = 0; unit < units; ++unit) {
-        int j, k;  // block; K tile number or -1: V
-        tc_unit<C::KT>(unit, j0, j, k);
-        if (k < 0 ? warp != 8 : warp != 10 + (turn++ & 1)) continue;
-        const int st = unit % C::NSLOT;
-        const uint32_t dst = ring0 + st * C::SLOT;
-        const int head0 = head * MAPS + (k < 0 ? slice * C::DV / D : k);
-        const int live = kv_end - j * kTcBlock;  // keys of the block that exist
-        // One lane for each box (TMA), each 16 tokens, or each of four times 32 tokens: where their rows are.
-        int64_t row[4] = {-1, -1, -1, -1};
-        unsigned bad[4] = {0, 0, 0, 0};
-        int phys = p.num_blocks, off = 0;  // the block behind the last is out of the map: zeros
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (whole && i) break;
-          const int in = by_tma ? lane * bt : whole ? 16 * lane : 32 * i + lane;
-          bool astray = false;
-          if (in < kTcBlock && in < live) {
-            const int token = j * kTcBlock + in, page = token / p.page;
-            const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
-            if ((unsigned)id < (unsigned)p.num_blocks) {
-              phys = id;
-              off = token - page * p.page;
-              row[i] = kv_row_offset(p, id, off, head0);
-            } else {
-              if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
-              astray = true;
-            }
-          }
-          bad[i] = __ballot_sync(kFull, astray);
-        }
-        if (whole && bad[0]) {  // a bit a box or 16 tokens -> a bit a token
-          const unsigned pieces = bad[0];
-          const int each = by_tma ? bt : 16;
-          for (int i = 0; i < 4; ++i) {
-            bad[i] = 0;
-            for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / each)) & 1u) << e;
-          }
-        }
-        if (!tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag)) break;
-        if (k == 0 && lane == 0)  // ahead of the block's scores
-          *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
-        if (by_tma) {
-          const bool tail = k < 0 && live < kTcBlock && live % bt != 0;  // V rows behind the last key in its box
-          const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
-          if (lane == 0) mbar_arrive_expect_tx(bar, 128 * 2 * (k < 0 ? C::DV : D));
-          if (lane > 0 && !tail) mbar_arrive(bar);
-          __syncwarp();
-          issued = unit;
-          if (lane < boxes) {
-            const uint32_t at = dst + lane * bt * 128;
-            if (k >= 0) {
-#pragma unroll
-              for (int c = 0; c < C::KH; ++c) tma_load_4d(at + c * (128 * 128), &tm_k, bar, c * 64, off, head0, phys);
-            } else {
-#pragma unroll
-              for (int c = 0; c < C::VC; ++c)
-                tma_load_4d(at + c * (128 * 128), &tm_v, bar, D == 64 ? 0 : c * 64, off, D == 64 ? head0 + c : head0, phys);
-            }
-          }
-          __syncwarp();
-          if (tail) {
-            tail_used = true;
-            if (!tc_wait(tail_bar, 0, p.status, abort_flag)) break;  // the one tail of this CTA
-            const int to = (live / bt + 1) * bt;
-            for (int i = lane; i < (to - live) * C::VC * 8; i += 32) {
-              const int r = live + i / 8 % (to - live), c = i / 8 / (to - live);
-              sts128(dst + tc_row(r, c) + (i & 7) * 16, make_uint4(0, 0, 0, 0));
-            }
-            fence_proxy_async();
-            mbar_arrive(full0 + 8 * st);
-          }
-        } else {
-          if (whole) {
-            if (k < 0) tc_copy_pages<C::VC, D>(dst, (const __half*)p.v, row[0], p.kv_st, p.kv_sh, live, lane);
-            else tc_copy_pages<C::KH, D>(dst, (const __half*)p.k, row[0], p.kv_st, p.kv_sh, live, lane);
-          } else {
-            if (k < 0) tc_copy_rows<C::VC, D>(dst, (const __half*)p.v, row, p.kv_sh, lane);
-            else tc_copy_rows<C::KH, D>(dst, (const __half*)p.k, row, p.kv_sh, lane);
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          fence_proxy_async();
-          mbar_arrive(full0 + 8 * st);
-        }
-      }
-      if (*abort_flag && by_tma) {  // boxes still in flight get a bounded chance to land
-        for (int u = issued; u >= 0 && u > issued - C::NSLOT; --u) {
-          int j, k;
-          tc_unit<C::KT>(u, j0, j, k);
-          if ((k < 0) == (warp == 8))
-            tc_drain(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u);
-        }
-        if (tail_used) tc_drain(tail_bar, 0);
-      }
-    }
-  }
   // ================================ widening warps (8-bit pages) =======================================
   // Four warps; a thread takes 16-byte pieces me, me + 128, .. of a tile's rows.  The pieces of the next unit
   // are on their way while this one's are widened and stored, and the block ids of a block are fetched a
   // block ahead (without that a tile cost two round trips to memory).
-  else if (warp >= 10) {
+  if (warp >= 12) {
     if constexpr (C::WIDEN) {
-      const int me = tid - 320;  // 0 .. 127
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_WIDEN));
+      const int me = tid - 384;  // 0 .. 127
       constexpr int PK = D / 16, PV = C::DV / 16;        // 16-byte pieces of a K and of a V row = of a thread
       constexpr int PM = PK > PV ? PK : PV;
       const int nb = jend - j0;
@@ -600,8 +502,9 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       };
       auto fetch_unit = [&](int j, int k, int64_t where, int64_t scale_where, uint4 (&x)[PM], __half (&sc)[SCALED ? C::KT + C::VH : 1]) {
         unsigned* mask = meta + 4 * (j & (kTcMetaRing - 1));
-        if (k < 0) tc_fetch<PV, D, PM>(p, tile.request, j, head * MAPS + slice * C::DV / D, p.v, whole, where, kv_end, mask, me, x);
-        else tc_fetch<PK, D, PM>(p, tile.request, j, head * MAPS + k, p.k, whole, where, kv_end, mask, me, x);
+        unsigned got;
+        if (k < 0) got = tc_fetch<PV, D, PM>(p, tile.request, j, head * MAPS + slice * C::DV / D, p.v, whole, where, kv_end, mask, me, x);
+        else got = tc_fetch<PK, D, PM>(p, tile.request, j, head * MAPS + k, p.k, whole, where, kv_end, mask, me, x);
         if constexpr (SCALED) {
           // the block's scales, K's and V's, with its first K tile: the softmax needs them ahead of V itself
           if (k == 0) {
@@ -611,17 +514,13 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             if (!whole) live = tc_place(p, tile.request, j * kTcBlock + me, kv_end, mask + me / 32, 1u << (me & 31), at) >= 0;
             at = (live ? at : 0) + head * MAPS;
 #pragma unroll
-            for (int z = 0; z < C::KT; ++z) {
-              const __half y = __ldg(p.k_scale + at + z);
-              sc[z] = live ? y : __ushort_as_half(0);
-            }
+            for (int z = 0; z < C::KT; ++z) sc[z] = __ldg(p.k_scale + at + z);
 #pragma unroll
-            for (int z = 0; z < C::VH; ++z) {
-              const __half y = __ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0));
-              sc[C::KT + z] = live ? y : __ushort_as_half(0);
-            }
+            for (int z = 0; z < C::VH; ++z) sc[C::KT + z] = __ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0));
+            if (live) got |= 1u << 31;
           }
         }
+        return got;
       };
       // where the tokens of block idj and of the one behind it lie
       int64_t s_here, s_next;
@@ -629,13 +528,14 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       int idj = j0;
       uint4 x[PM];
       __half sc[SCALED ? C::KT + C::VH : 1];
-      if (units > 0) fetch_unit(j0, 0, here, s_here, x, sc);
+      unsigned live = units > 0 ? fetch_unit(j0, 0, here, s_here, x, sc) : 0;  // pieces of x, and bit 31: of sc
       bool ok = true;
       for (int unit = 0; unit < units && ok; ++unit) {
         int j, k;
         tc_unit<C::KT>(unit, j0, j, k);
         uint4 nx[PM];
         __half nsc[SCALED ? C::KT + C::VH : 1];
+        unsigned nlive = 0;
         if (unit + 1 < units) {
           int j2, k2;
           tc_unit<C::KT>(unit + 1, j0, j2, k2);
@@ -648,7 +548,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             if (me < 4) meta[4 * ((idj + 1 + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;
             next = locate(idj + 1, s_next);
           }
-          fetch_unit(j2, k2, j2 > idj ? next : here, j2 > idj ? s_next : s_here, nx, nsc);
+          nlive = fetch_unit(j2, k2, j2 > idj ? next : here, j2 > idj ? s_next : s_here, nx, nsc);
         }
         const int st = unit % C::NSLOT;
         const uint32_t dst = ring0 + st * C::SLOT;
@@ -660,10 +560,11 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           if (i >= pieces) continue;
           const int n = me + i * 128, r = n / pieces, c = n % pieces;
           const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          const uint32_t keep = (live >> i) & 1 ? 0xffffffffu : 0u;
           uint32_t h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t y = KV == PD_KV_I8 ? w[e] ^ 0x80808080u : w[e];
+            const uint32_t y = KV == PD_KV_I8 ? (w[e] & keep) ^ 0x80808080u : w[e] & keep;
             h[2 * e] = cvt_pair<KV>(y, false);
             h[2 * e + 1] = cvt_pair<KV>(y, true);
           }
@@ -682,13 +583,15 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           if (k == 0) {
 #pragma unroll
             for (int z = 0; z < C::KT + C::VH; ++z)
-              scales[(j % C::SCALE_RING) * C::SCALE_FLOATS + z * 128 + me] = __half2float(sc[z]) * (z < C::KT ? 1.f : kBoost);
+              scales[(j % C::SCALE_RING) * C::SCALE_FLOATS + z * 128 + me] =
+                  live >> 31 ? __half2float(sc[z]) * (z < C::KT ? 1.f : kBoost) : 0.f;
           }
         }
         fence_proxy_async();
         mbar_arrive(full0 + 8 * st);
 #pragma unroll
         for (int i = 0; i < PM; ++i) x[i] = nx[i];
+        live = nlive;
         if constexpr (SCALED) {
 #pragma unroll
           for (int z = 0; z < C::KT + C::VH; ++z) sc[z] = nsc[z];
@@ -696,125 +599,237 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       }
     }
   }
-  // ================================ matrix units ======================================================
-  else if (warp == 9) {
-    constexpr uint32_t id_s = tc_idesc(C::BF16, 128, false);
-    constexpr uint32_t id_o = tc_idesc(C::BF16, C::DV / C::NP, true);
-    uint32_t mine;
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(mine));
-    bool ok = true;
-    auto wait_bar = [&](uint32_t bar, uint32_t parity) {
-      return tc_wait(bar, parity, p.status, abort_flag);
-    };
-    auto scores = [&](int t, int kslot) {  // S_t = Q_t K^T
-      const uint64_t qd = tc_desc(q0 + t * C::QTILE, 1024, 0), kd = tc_desc(ring0 + kslot * C::SLOT, 1024, 0);
+  // ================================ the third group: loaders and the matrix units' warp =================
+  else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_THIRD));
+    // ================================ loaders (16-bit pages) =============================================
+    // V's tiles: warp 8; K's: warps 10 and 11 in turn.
+    if constexpr (!C::WIDEN) {
+      if (warp != 9) {
+        const int nb = jend - j0;
+        const int units = nb > 0 ? nb * (C::KT + 1) : 0;
+        const bool whole = p.page % 16 == 0;                 // 16 tokens lie in one page
+        const bool by_tma = whole && (warp == 8 || p.page % 64 == 0);
+        const int bt = tp.box_tokens, boxes = kTcBlock / bt;
+        int turn = 0, issued = -1;
+        bool tail_used = false;
+        for (int unit = 0; unit < units; ++unit) {
+          int j, k;  // block; K tile number or -1: V
+          tc_unit<C::KT>(unit, j0, j, k);
+          if (k < 0 ? warp != 8 : warp != 10 + (turn++ & 1)) continue;
+          const int st = unit % C::NSLOT;
+          const uint32_t dst = ring0 + st * C::SLOT;
+          const int head0 = head * MAPS + (k < 0 ? slice * C::DV / D : k);
+          const int live = kv_end - j * kTcBlock;  // keys of the block that exist
+          // One lane for each box (TMA), each 16 tokens, or each of four times 32 tokens: where their rows are.
+          int64_t row[4] = {-1, -1, -1, -1};
+          unsigned bad[4] = {0, 0, 0, 0};
+          int phys = p.num_blocks, off = 0;  // the block behind the last is out of the map: zeros
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks)
-        tc_mma_ss(tmem + t * 128, qd + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4),
-                  kd + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4), id_s, ks > 0, mine);
-      tc_commit(s_full + 8 * t, mine);
-    };
-    auto values = [&](int t, int vslot, bool first, int half) {  // O_t (+)= P_t V, 64 keys
-      const uint64_t vd = tc_desc(ring0 + vslot * C::SLOT, 1024, 128 * 128);
-#pragma unroll
-      for (int z = 0; z < C::NP; ++z) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int ks = 4 * half + k;
-          const uint32_t pa = C::NP == 1 ? 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks % 2);
-          tc_mma_ts(tmem + 256 + t * 128 + z * 64, tmem + t * 128 + pa, vd + ((z * (128 * 128) + ks * 2048) >> 4), id_o,
-                    !first || ks > 0, mine);
-        }
-      }
-    };
-    if (jend > j0) {
-      ok = wait_bar(q_full, 0);
-      // unit u lives in slot u % NSLOT; slot and phase of the next unit are counted along
-      int slot = 0;
-      uint32_t phase = 0;
-      auto step = [&] {
-        if (++slot == C::NSLOT) {
-          slot = 0;
-          phase ^= 1;
-        }
-      };
-      // the first block's scores
-      if (ok) ok = wait_bar(full0, 0);
-      if (ok) {
-        tc_fence_after();
-        if (end[0] > j0) scores(0, 0);
-        step();
-        if constexpr (MAPS == 2) {
-          ok = wait_bar(full0 + 8, 0);
-          if (ok) {
-            tc_fence_after();
-            scores(1, 1);
-            tc_commit(empty0, mine);
-            tc_commit(empty0 + 8, mine);
-          }
-          step();
-        } else {
-          if (end[1] > j0) scores(1, 0);
-          tc_commit(empty0, mine);
-        }
-      }
-      for (int j = j0; j < jend && ok; ++j) {
-        const uint32_t par = (uint32_t)(j - j0) & 1u;
-        const bool more = j + 1 < jend;
-        const int vslot = slot;
-        const uint32_t vphase = phase;
-        int kslot[C::KT];
-        uint32_t kphase[C::KT];
-        step();
-        if (more) {
-#pragma unroll
-          for (int k = 0; k < C::KT; ++k) {
-            kslot[k] = slot;
-            kphase[k] = phase;
-            step();
-          }
-        }
-        ok = wait_bar(full0 + 8 * vslot, vphase);
-        if (more && C::KT == 1 && ok) ok = wait_bar(full0 + 8 * kslot[0], kphase[0]);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= end[t] || !ok) continue;
-          ok = wait_bar(p_full + 16 * t, par);
-          if (!ok) break;
-          tc_fence_after();
-          values(t, vslot, j == j0, 0);
-          ok = wait_bar(p_full + 16 * t + 8, par);
-          if (!ok) break;
-          tc_fence_after();
-          values(t, vslot, j == j0, 1);
-          if (j + 1 < end[t]) {
-            if constexpr (C::KT == 2) {
-              ok = wait_bar(full0 + 8 * kslot[t], kphase[t]);
-              if (!ok) break;
-              tc_fence_after();
+          for (int i = 0; i < 4; ++i) {
+            if (whole && i) break;
+            const int in = by_tma ? lane * bt : whole ? 16 * lane : 32 * i + lane;
+            bool astray = false;
+            if (in < kTcBlock && in < live) {
+              const int token = j * kTcBlock + in, page = token / p.page;
+              const int id = __ldg(p.block_table + (int64_t)tile.request * p.bt_stride + page);
+              if ((unsigned)id < (unsigned)p.num_blocks) {
+                phys = id;
+                off = token - page * p.page;
+                row[i] = kv_row_offset(p, id, off, head0);
+              } else {
+                if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
+                astray = true;
+              }
             }
-            scores(t, kslot[C::KT == 2 ? t : 0]);
+            bad[i] = __ballot_sync(kFull, astray);
+          }
+          if (whole && bad[0]) {  // a bit a box or 16 tokens -> a bit a token
+            const unsigned pieces = bad[0];
+            const int each = by_tma ? bt : 16;
+            for (int i = 0; i < 4; ++i) {
+              bad[i] = 0;
+              for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / each)) & 1u) << e;
+            }
+          }
+          if (!tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag)) break;
+          if (k == 0 && lane == 0)  // ahead of the block's scores
+            *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
+          if (by_tma) {
+            const bool tail = k < 0 && live < kTcBlock && live % bt != 0;  // V rows behind the last key in its box
+            const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
+            if (lane == 0) mbar_arrive_expect_tx(bar, 128 * 2 * (k < 0 ? C::DV : D));
+            if (lane > 0 && !tail) mbar_arrive(bar);
+            __syncwarp();
+            issued = unit;
+            if (lane < boxes) {
+              const uint32_t at = dst + lane * bt * 128;
+              if (k >= 0) {
+#pragma unroll
+                for (int c = 0; c < C::KH; ++c) tma_load_4d(at + c * (128 * 128), &tm_k, bar, c * 64, off, head0, phys);
+              } else {
+#pragma unroll
+                for (int c = 0; c < C::VC; ++c)
+                  tma_load_4d(at + c * (128 * 128), &tm_v, bar, D == 64 ? 0 : c * 64, off, D == 64 ? head0 + c : head0, phys);
+              }
+            }
+            __syncwarp();
+            if (tail) {
+              tail_used = true;
+              if (!tc_wait(tail_bar, 0, p.status, abort_flag)) break;  // the one tail of this CTA
+              const int to = (live / bt + 1) * bt;
+              for (int i = lane; i < (to - live) * C::VC * 8; i += 32) {
+                const int r = live + i / 8 % (to - live), c = i / 8 / (to - live);
+                sts128(dst + tc_row(r, c) + (i & 7) * 16, make_uint4(0, 0, 0, 0));
+              }
+              fence_proxy_async();
+              mbar_arrive(full0 + 8 * st);
+            }
           } else {
-            tc_commit(o_done + 8 * t, mine);
+            if (whole) {
+              if (k < 0) tc_copy_pages<C::VC, D>(dst, (const __half*)p.v, row[0], p.kv_st, p.kv_sh, live, lane);
+              else tc_copy_pages<C::KH, D>(dst, (const __half*)p.k, row[0], p.kv_st, p.kv_sh, live, lane);
+            } else {
+              if (k < 0) tc_copy_rows<C::VC, D>(dst, (const __half*)p.v, row, p.kv_sh, lane);
+              else tc_copy_rows<C::KH, D>(dst, (const __half*)p.k, row, p.kv_sh, lane);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async();
+            mbar_arrive(full0 + 8 * st);
           }
         }
-        if (!ok) break;
-        // both tiles' products with these tiles are issued: their slots are free when they are done
-        tc_commit(empty0 + 8 * vslot, mine);
-        if (more) {
-#pragma unroll
-          for (int k = 0; k < C::KT; ++k) tc_commit(empty0 + 8 * kslot[k], mine);
+        if (*abort_flag && by_tma) {  // boxes still in flight get a bounded chance to land
+          for (int u = issued; u >= 0 && u > issued - C::NSLOT; --u) {
+            int j, k;
+            tc_unit<C::KT>(u, j0, j, k);
+            if ((k < 0) == (warp == 8))
+              tc_drain(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u);
+          }
+          if (tail_used) tc_drain(tail_bar, 0);
         }
-      }
-      if (!ok) {  // products in flight get a bounded chance to end before tensor memory is freed
-        tc_commit(drain_bar, mine);
-        tc_drain(drain_bar, 0);
       }
     }
-    __syncwarp();
+  // ================================ matrix units ======================================================
+    if (warp == 9) {
+      constexpr uint32_t id_s = tc_idesc(C::BF16, 128, false);
+      constexpr uint32_t id_o = tc_idesc(C::BF16, C::DV / C::NP, true);
+      uint32_t mine;
+      asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(mine));
+      bool ok = true;
+      auto wait_bar = [&](uint32_t bar, uint32_t parity) {
+        return tc_wait(bar, parity, p.status, abort_flag);
+      };
+      auto scores = [&](int t, int kslot) {  // S_t = Q_t K^T
+        const uint64_t qd = tc_desc(q0 + t * C::QTILE, 1024, 0), kd = tc_desc(ring0 + kslot * C::SLOT, 1024, 0);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          tc_mma_ss(tmem + t * 128, qd + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4),
+                    kd + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4), id_s, ks > 0, mine);
+        tc_commit(s_full + 8 * t, mine);
+      };
+      auto values = [&](int t, int vslot, bool first, int half) {  // O_t (+)= P_t V, 64 keys
+        const uint64_t vd = tc_desc(ring0 + vslot * C::SLOT, 1024, 128 * 128);
+#pragma unroll
+        for (int z = 0; z < C::NP; ++z) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int ks = 4 * half + k;
+            const uint32_t pa = C::NP == 1 ? 8 * ks : 32 * (ks / 2) + 16 * z + 8 * (ks % 2);
+            tc_mma_ts(tmem + 256 + t * 128 + z * 64, tmem + t * 128 + pa, vd + ((z * (128 * 128) + ks * 2048) >> 4), id_o,
+                      !first || ks > 0, mine);
+          }
+        }
+      };
+      if (jend > j0) {
+        ok = wait_bar(q_full, 0);
+        // unit u lives in slot u % NSLOT; slot and phase of the next unit are counted along
+        int slot = 0;
+        uint32_t phase = 0;
+        auto step = [&] {
+          if (++slot == C::NSLOT) {
+            slot = 0;
+            phase ^= 1;
+          }
+        };
+        // the first block's scores
+        if (ok) ok = wait_bar(full0, 0);
+        if (ok) {
+          tc_fence_after();
+          if (end[0] > j0) scores(0, 0);
+          step();
+          if constexpr (MAPS == 2) {
+            ok = wait_bar(full0 + 8, 0);
+            if (ok) {
+              tc_fence_after();
+              scores(1, 1);
+              tc_commit(empty0, mine);
+              tc_commit(empty0 + 8, mine);
+            }
+            step();
+          } else {
+            if (end[1] > j0) scores(1, 0);
+            tc_commit(empty0, mine);
+          }
+        }
+        for (int j = j0; j < jend && ok; ++j) {
+          const uint32_t par = (uint32_t)(j - j0) & 1u;
+          const bool more = j + 1 < jend;
+          const int vslot = slot;
+          const uint32_t vphase = phase;
+          int kslot[C::KT];
+          uint32_t kphase[C::KT];
+          step();
+          if (more) {
+#pragma unroll
+            for (int k = 0; k < C::KT; ++k) {
+              kslot[k] = slot;
+              kphase[k] = phase;
+              step();
+            }
+          }
+          ok = wait_bar(full0 + 8 * vslot, vphase);
+          if (more && C::KT == 1 && ok) ok = wait_bar(full0 + 8 * kslot[0], kphase[0]);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= end[t] || !ok) continue;
+            ok = wait_bar(p_full + 16 * t, par);
+            if (!ok) break;
+            tc_fence_after();
+            values(t, vslot, j == j0, 0);
+            ok = wait_bar(p_full + 16 * t + 8, par);
+            if (!ok) break;
+            tc_fence_after();
+            values(t, vslot, j == j0, 1);
+            if (j + 1 < end[t]) {
+              if constexpr (C::KT == 2) {
+                ok = wait_bar(full0 + 8 * kslot[t], kphase[t]);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              scores(t, kslot[C::KT == 2 ? t : 0]);
+            } else {
+              tc_commit(o_done + 8 * t, mine);
+            }
+          }
+          if (!ok) break;
+          // both tiles' products with these tiles are issued: their slots are free when they are done
+          tc_commit(empty0 + 8 * vslot, mine);
+          if (more) {
+#pragma unroll
+            for (int k = 0; k < C::KT; ++k) tc_commit(empty0 + 8 * kslot[k], mine);
+          }
+        }
+        if (!ok) {  // products in flight get a bounded chance to end before tensor memory is freed
+          tc_commit(drain_bar, mine);
+          tc_drain(drain_bar, 0);
+        }
+      }
+      __syncwarp();
+    }
   }
   // ================================ softmax ============================================================
   else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
     const int t = warp >> 2;            // tile
     const int me = tid & 127;           // row of the tile
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
@@ -878,23 +893,15 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             if (c0 + c >= room || ((astray >> c) & 1)) x[c] = -INFINITY;
         }
       };
-      // The row's maximum; 16-bit pages keep the 128 scores in registers, 8-bit ones (more warps, fewer
-      // registers) read them from tensor memory again.
-      constexpr bool HOLD = !C::WIDEN;
-      float x[HOLD ? 128 : 32];
+      // the row's scores, in registers from here on, and their maximum
+      float x[128];
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if constexpr (HOLD) {
 #pragma unroll
-        for (int c0 = 0; c0 < 128; c0 += 32) tc_ld32(s_at + c0, x + c0);
-        tc_wait_ld();
-      }
+      for (int c0 = 0; c0 < 128; c0 += 32) tc_ld32(s_at + c0, x + c0);
+      tc_wait_ld();
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 32) {
-        float* y = HOLD ? x + c0 : x;
-        if constexpr (!HOLD) {
-          tc_ld32(s_at + c0, y);
-          tc_wait_ld();
-        }
+        float* y = x + c0;
         shape_scores(y, c0);
 #pragma unroll
         for (int c = 0; c < 32; c += 2) mx[(c >> 1) & 3] = tc_max3(mx[(c >> 1) & 3], y[c], y[c + 1]);
@@ -921,12 +928,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 32) {
-        float* y = HOLD ? x + c0 : x;
-        if constexpr (!HOLD) {
-          tc_ld32(s_at + c0, y);
-          tc_wait_ld();
-          shape_scores(y, c0);
-        }
+        float* y = x + c0;
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           tc_fma2(y[c], y[c + 1], p.scale_log2, -from);
