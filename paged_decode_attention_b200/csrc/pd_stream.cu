@@ -428,7 +428,11 @@ int diff_stream_run(const PdPrefillArgs* a, int sm_count) {
   if (!encode_tensor_map_in_place(map_key(&d, s, d.k_cache), &mk) ||
       !encode_tensor_map_in_place(map_key(&d, s, d.v_cache), &mv))
     return PD_ERR_CUDA;
-  return launch_stream(&d, p, s, sm, wl, (char*)a->workspace, mk, mv, sm_count, false, nullptr, &t);
+  // Where every request is sure to be dealt whole (the block table has no room for longer ones), the pairs
+  // meet in shared memory and nothing in the scratch has to start at zero.
+  const bool whole = (int64_t)a->max_blocks_per_seq * a->block_size <= (int64_t)kWholeTiles * kTileTokens &&
+                     s.nvseq <= sm_count * s.wpc;
+  return launch_stream(&d, p, s, sm, wl, (char*)a->workspace, mk, mv, sm_count, whole, nullptr, &t);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -1040,6 +1040,9 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     prefix[0] = 0;
     nonempty[0] = 0;
     *abort_flag = 0;
+    // requests dealt whole have no boundaries; a differential pair's two warps, which are then in this CTA,
+    // count their arrivals there
+    if constexpr (MAPS == 2) bound[0] = bound[1] = bound[2] = bound[3] = 0;
     // step counter of this rank's exchange buffer: its parity names the slots of this step
     *push_step = pushing ? *reinterpret_cast<volatile uint32_t*>(sp.push.peers.buf[sp.push.rank]) : 0u;
   }
@@ -1608,7 +1611,10 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
         }
       } else {
         int last = 0;
-        if (lane == 0) {
+        if (MAPS == 2 && dealt_whole) {
+          static_assert(MAPS == 1 || WPC * HB / 2 <= 4, "one counter for each pair of the CTA");
+          if (lane == 0) last = atomicAdd(&bound[wl * (HB / 2) + role / 2], 1) == 1;
+        } else if (lane == 0) {
           int expected = 0;
           if constexpr (MAPS == 2) expected = 2 * nseg;  // always unsplit
           else for_each_segment(prefix, cm, v0, sp.splits, [&](int) { ++expected; });

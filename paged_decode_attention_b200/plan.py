@@ -89,13 +89,9 @@ def plan_step(block_table: torch.Tensor, context_lens: torch.Tensor, new_tokens:
     free = _vector(free_blocks, "free_blocks", i32, None, index)
     nfree = _vector(num_free, "num_free", i32, 1, index)
     if out is None:
-        dev = block_table.device
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-        positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-        starts, lens, left = torch.empty(2 * b + 2, dtype=i32, device=dev).split((b + 1, b, 1))
-        out = StepPlan(slots, positions, starts, lens, left)
-        at = starts.data_ptr()
-        ptrs = (slots.data_ptr(), positions.data_ptr(), at, at + 4 * (b + 1), at + 4 * (2 * b + 1))
+        make = num_free.new_empty
+        out = StepPlan(make(num_tokens, dtype=torch.int64), make(num_tokens, dtype=torch.int64), make(b + 1), make(b), make(1))
+        ptrs = [t.data_ptr() for t in out]
     else:
         ptrs = (_vector(out.slot_mapping, "out.slot_mapping", torch.int64, num_tokens, index),
                 _vector(out.positions, "out.positions", torch.int64, num_tokens, index),

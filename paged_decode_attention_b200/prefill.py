@@ -147,7 +147,7 @@ def _run(entry: str, q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor | N
         raise _cabi.NativeLibraryError(f"{entry} runs on CUDA tensors only; there is no CPU path")
     index = q.get_device()
     if out is None:
-        out = torch.empty((q.shape[0], q.shape[1], maps * q.shape[-1]), dtype=q.dtype, device=q.device)
+        out = q.new_empty((q.shape[0], q.shape[1], maps * q.shape[-1]))
     values = build_prefill_args(q, cache, out, query_start_loc, maps=maps, stream=_current_stream(index), **kw)
     if q.shape[0] == 0 or cache.batch == 0:
         return out
@@ -160,7 +160,7 @@ def _run(entry: str, q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor | N
     if need.value:
         # Scratch of this call alone, from torch's allocator: ordered by the stream, and inside a
         # capture a part of that graph, so no two graphs or streams share it.
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need.value, dtype=torch.uint8)
         block = block[:_SCRATCH_AT] + _SCRATCH.pack(ws.data_ptr(), need.value) + block[_SCRATCH_AT + _SCRATCH.size:]
     rc = _call_on_index(index, getattr(lib, entry), block)
     if rc != 0:
