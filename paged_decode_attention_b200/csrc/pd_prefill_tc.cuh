@@ -77,7 +77,7 @@ struct TcCfg {
   static constexpr int REGS_SOFTMAX = WIDEN ? 176 : 200, REGS_THIRD = WIDEN ? 56 : 104, REGS_WIDEN = 104;
   static_assert(WIDEN ? 2 * REGS_SOFTMAX + REGS_THIRD + REGS_WIDEN <= 4 * 128 : 2 * REGS_SOFTMAX + REGS_THIRD <= 3 * 168, "registers");
   static constexpr int THREADS = WARPS * 32;
-  static_assert(NSLOT >= 3 && SMEM <= kTcSmem, "shared memory");
+  static_assert(NSLOT >= (WIDEN ? 3 : 4) && SMEM <= kTcSmem, "shared memory; a loader's own units are at most four apart");
 };
 
 struct TcParams {
@@ -231,28 +231,29 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
   }
 }
 
-// 128 rows of PIECES * 64 columns into a tile; row[i] of lane l is the offset of row 32 i + l's first column
-// (-1: zeros).  Pieces beyond a head's D columns belong to the next head.
-template <int PIECES, int D>
+// Rows of PIECES * 64 columns into a tile, the first `PARTS`-th of its 128 or the `part`-th; row[i] of lane l is the
+// offset of row 32 i + l's first column (-1: zeros).  Pieces beyond a head's D columns belong to the next head.
+template <int PIECES, int D, int PARTS>
 __device__ __forceinline__ void tc_copy_rows(uint32_t dst, const __half* cache, const int64_t (&row)[4], int64_t head_stride,
-                                             int lane) {
+                                             int part, int lane) {
   constexpr int CH = PIECES * 8;  // 16-byte chunks, and lanes, of a row
   constexpr int RPI = 32 / CH;    // rows of one warp-wide copy
   const int c = lane % CH, rr = lane / CH, piece = c / 8;
   const __half* mine = cache + (D == 64 && piece ? head_stride : 0) + (D == 64 ? c % 8 : c) * 8;
 #pragma unroll
-  for (int i = 0; i < 128 / RPI; ++i) {
-    const int r = i * RPI + rr;
-    const int64_t at = __shfl_sync(0xffffffffu, row[i * RPI / 32], r & 31);
+  for (int n = 0; n < 128 / PARTS / RPI; ++n) {
+    const int r = part * (128 / PARTS) + n * RPI + rr;
+    const int64_t mine_of = PARTS == 1 ? row[n * RPI / 32] : part ? row[2 + n * RPI / 32] : row[n * RPI / 32];
+    const int64_t at = __shfl_sync(0xffffffffu, mine_of, r & 31);
     cp_async16(dst + tc_row(r, piece) + (((c & 7) ^ (r & 7)) << 4), at >= 0 ? mine + at : cache, at >= 0);
   }
 }
 
 // The same for pages of a multiple of 16 tokens: a piece of 16 tokens lies in one page, so its rows are a
 // stride apart.  `at` of lane g is the offset of token 16 g's row (-1: zeros), `live` tokens exist.
-template <int PIECES, int D>
+template <int PIECES, int D, int PARTS>
 __device__ __forceinline__ void tc_copy_pages(uint32_t dst, const __half* cache, int64_t at, int64_t token_stride,
-                                              int64_t head_stride, int live, int lane) {
+                                              int64_t head_stride, int live, int part, int lane) {
   constexpr int CH = PIECES * 8, RPI = 32 / CH;
   const int c = lane % CH, rr = lane / CH, piece = c / 8;
   const __half* mine = cache + (D == 64 && piece ? head_stride : 0) + (D == 64 ? c % 8 : c) * 8 + rr * token_stride;
@@ -263,7 +264,8 @@ __device__ __forceinline__ void tc_copy_pages(uint32_t dst, const __half* cache,
     to[i] = dst + tc_row(r, piece) + (((c & 7) ^ r) << 4);
   }
 #pragma unroll
-  for (int g = 0; g < 8; ++g) {
+  for (int n = 0; n < 8 / PARTS; ++n) {
+    const int g = part * (8 / PARTS) + n;
     const int64_t off = __shfl_sync(0xffffffffu, at, g);
     const __half* src = off >= 0 ? mine + off : cache;
     const int64_t step = off >= 0 ? RPI * token_stride : 0;
@@ -603,20 +605,25 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_THIRD));
     // ================================ loaders (16-bit pages) =============================================
-    // V's tiles: warp 8; K's: warps 10 and 11 in turn.
+    // V's tiles: warp 8; K's: warps 10 and 11.
     if constexpr (!C::WIDEN) {
       if (warp != 9) {
         const int nb = jend - j0;
         const int units = nb > 0 ? nb * (C::KT + 1) : 0;
         const bool whole = p.page % 16 == 0;                 // 16 tokens lie in one page
-        const bool by_tma = whole && (warp == 8 || p.page % 64 == 0);
+        const bool wide = p.page % 64 == 0;                  // boxes of 64 tokens and more
         const int bt = tp.box_tokens, boxes = kTcBlock / bt;
-        int turn = 0, issued = -1;
+        int issued = -1;
         bool tail_used = false;
         for (int unit = 0; unit < units; ++unit) {
           int j, k;  // block; K tile number or -1: V
           tc_unit<C::KT>(unit, j0, j, k);
-          if (k < 0 ? warp != 8 : warp != 10 + (turn++ & 1)) continue;
+          const bool by_tma = whole && (k < 0 || wide);
+          // Who takes it: V warp 8; two K tiles of a block warps 10 and 11; one K tile, by TMA, the two in turn, by
+          // copies each half of its rows.  Nobody may skip more than NSLOT units: a slot's barrier tells a phase
+          // only from the one before, and a warp knows that the use before last is over by its own last unit.
+          const bool halves = C::KT == 1 && k == 0 && !by_tma;
+          if (k < 0 ? warp != 8 : warp == 8 || (!halves && warp != 10 + (C::KT == 2 ? k : (j - j0) & 1))) continue;
           const int st = unit % C::NSLOT;
           const uint32_t dst = ring0 + st * C::SLOT;
           const int head0 = head * MAPS + (k < 0 ? slice * C::DV / D : k);
@@ -653,7 +660,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             }
           }
           if (!tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag)) break;
-          if (k == 0 && lane == 0)  // ahead of the block's scores
+          if (k == 0 && lane == 0 && !(halves && warp == 11))  // ahead of the block's scores
             *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
           if (by_tma) {
             const bool tail = k < 0 && live < kTcBlock && live % bt != 0;  // V rows behind the last key in its box
@@ -686,25 +693,20 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
               mbar_arrive(full0 + 8 * st);
             }
           } else {
-            if (whole) {
-              if (k < 0) tc_copy_pages<C::VC, D>(dst, (const __half*)p.v, row[0], p.kv_st, p.kv_sh, live, lane);
-              else tc_copy_pages<C::KH, D>(dst, (const __half*)p.k, row[0], p.kv_st, p.kv_sh, live, lane);
-            } else {
-              if (k < 0) tc_copy_rows<C::VC, D>(dst, (const __half*)p.v, row, p.kv_sh, lane);
-              else tc_copy_rows<C::KH, D>(dst, (const __half*)p.k, row, p.kv_sh, lane);
-            }
+            constexpr int PARTS = C::KT == 1 ? 2 : 1;
+            const int part = PARTS == 2 ? warp - 10 : 0;
+            if (whole) tc_copy_pages<C::KH, D, PARTS>(dst, (const __half*)p.k, row[0], p.kv_st, p.kv_sh, live, part, lane);
+            else if (k < 0) tc_copy_rows<C::VC, D, 1>(dst, (const __half*)p.v, row, p.kv_sh, 0, lane);
+            else tc_copy_rows<C::KH, D, PARTS>(dst, (const __half*)p.k, row, p.kv_sh, part, lane);
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
-            mbar_arrive(full0 + 8 * st);
+            __syncwarp();
+            if (!halves || lane < 16) mbar_arrive(full0 + 8 * st);  // 32 arrivals a unit
           }
         }
-        if (*abort_flag && by_tma) {  // boxes still in flight get a bounded chance to land
-          for (int u = issued; u >= 0 && u > issued - C::NSLOT; --u) {
-            int j, k;
-            tc_unit<C::KT>(u, j0, j, k);
-            if ((k < 0) == (warp == 8))
-              tc_drain(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u);
-          }
+        if (*abort_flag && issued >= 0) {  // boxes still in flight get a bounded chance to land
+          for (int u = issued; u >= 0 && u > issued - C::NSLOT; --u)
+            tc_drain(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u);
           if (tail_used) tc_drain(tail_bar, 0);
         }
       }
