@@ -18,12 +18,11 @@
 // 16-bit pairs and is read by the second product from tensor memory; shared memory holds Q and a
 // ring of K and V tiles in the 128-byte swizzle.
 //
-// Three warps fill the ring.  With pages of a multiple of 64 tokens everything comes by TMA.  TMA runs a
-// 16-token box (2 KB) in about 150 cycles, though, and a block has 32 of those, more than its products
-// take; so with smaller pages V comes by TMA and K by 16-byte asynchronous copies of two other warps, side
-// by side (8192 tokens, pages of 16: all TMA 634 us, all copies 749 us).  Copies also serve pages that are
-// no multiple of 16, and leave out what lies behind the last key; V's rows there are cleared behind the
-// copy, because zero times the NaN that a page may hold would stay.
+// Three warps fill the ring, a lane for each TMA box of up to 128 tokens of a page and 64 columns.  What
+// such boxes cost is their number: 32 of 16 tokens a block keep pace with the products only when the waits
+// leave the SM alone and several warps issue (8192 tokens, pages of 16: 473 us, pages of 128: 457).  Pages
+// that are no multiple of 16 tokens come by 16-byte asynchronous copies, row by row.  V's rows behind the last
+// key are cleared behind the copy, because zero times the NaN that a page may hold would stay.
 //
 // The maximum that P refers to may lag behind the true one by kLag (2^3 or 2^8 at most): O is then not
 // rescaled for every small rise.  It cancels in O / l; l and O are 32-bit.
@@ -231,50 +230,20 @@ __device__ __forceinline__ uint32_t tc_pack(float lo, float hi) {
   }
 }
 
-// Rows of PIECES * 64 columns into a tile, the first `PARTS`-th of its 128 or the `part`-th; row[i] of lane l is the
-// offset of row 32 i + l's first column (-1: zeros).  Pieces beyond a head's D columns belong to the next head.
-template <int PIECES, int D, int PARTS>
+// 128 rows of PIECES * 64 columns into a tile; row[i] of lane l is the offset of row 32 i + l's first column
+// (-1: zeros).  Pieces beyond a head's D columns belong to the next head.
+template <int PIECES, int D>
 __device__ __forceinline__ void tc_copy_rows(uint32_t dst, const __half* cache, const int64_t (&row)[4], int64_t head_stride,
-                                             int part, int lane) {
+                                             int lane) {
   constexpr int CH = PIECES * 8;  // 16-byte chunks, and lanes, of a row
   constexpr int RPI = 32 / CH;    // rows of one warp-wide copy
   const int c = lane % CH, rr = lane / CH, piece = c / 8;
   const __half* mine = cache + (D == 64 && piece ? head_stride : 0) + (D == 64 ? c % 8 : c) * 8;
 #pragma unroll
-  for (int n = 0; n < 128 / PARTS / RPI; ++n) {
-    const int r = part * (128 / PARTS) + n * RPI + rr;
-    const int64_t mine_of = PARTS == 1 ? row[n * RPI / 32] : part ? row[2 + n * RPI / 32] : row[n * RPI / 32];
-    const int64_t at = __shfl_sync(0xffffffffu, mine_of, r & 31);
-    cp_async16(dst + tc_row(r, piece) + (((c & 7) ^ (r & 7)) << 4), at >= 0 ? mine + at : cache, at >= 0);
-  }
-}
-
-// The same for pages of a multiple of 16 tokens: a piece of 16 tokens lies in one page, so its rows are a
-// stride apart.  `at` of lane g is the offset of token 16 g's row (-1: zeros), `live` tokens exist.
-template <int PIECES, int D, int PARTS>
-__device__ __forceinline__ void tc_copy_pages(uint32_t dst, const __half* cache, int64_t at, int64_t token_stride,
-                                              int64_t head_stride, int live, int part, int lane) {
-  constexpr int CH = PIECES * 8, RPI = 32 / CH;
-  const int c = lane % CH, rr = lane / CH, piece = c / 8;
-  const __half* mine = cache + (D == 64 && piece ? head_stride : 0) + (D == 64 ? c % 8 : c) * 8 + rr * token_stride;
-  uint32_t to[8 / RPI];  // where the lane's rows of an 8-row group go
-#pragma unroll
-  for (int i = 0; i < 8 / RPI; ++i) {
+  for (int i = 0; i < 128 / RPI; ++i) {
     const int r = i * RPI + rr;
-    to[i] = dst + tc_row(r, piece) + (((c & 7) ^ r) << 4);
-  }
-#pragma unroll
-  for (int n = 0; n < 8 / PARTS; ++n) {
-    const int g = part * (8 / PARTS) + n;
-    const int64_t off = __shfl_sync(0xffffffffu, at, g);
-    const __half* src = off >= 0 ? mine + off : cache;
-    const int64_t step = off >= 0 ? RPI * token_stride : 0;
-    const int rows = off >= 0 ? live - 16 * g - rr : 0;  // of this lane: row i * RPI exists when below
-#pragma unroll
-    for (int i = 0; i < 16 / RPI; ++i) {
-      cp_async16(to[i % (8 / RPI)] + (2 * g + i / (8 / RPI)) * 1024, src, i * RPI < rows);
-      src += step;
-    }
+    const int64_t at = __shfl_sync(0xffffffffu, row[i * RPI / 32], r & 31);
+    cp_async16(dst + tc_row(r, piece) + (((c & 7) ^ (r & 7)) << 4), at >= 0 ? mine + at : cache, at >= 0);
   }
 }
 
@@ -611,31 +580,28 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         const int nb = jend - j0;
         const int units = nb > 0 ? nb * (C::KT + 1) : 0;
         const bool whole = p.page % 16 == 0;                 // 16 tokens lie in one page
-        const bool wide = p.page % 64 == 0;                  // boxes of 64 tokens and more
         const int bt = tp.box_tokens, boxes = kTcBlock / bt;
         int issued = -1;
         bool tail_used = false;
         for (int unit = 0; unit < units; ++unit) {
           int j, k;  // block; K tile number or -1: V
           tc_unit<C::KT>(unit, j0, j, k);
-          const bool by_tma = whole && (k < 0 || wide);
-          // Who takes it: V warp 8; two K tiles of a block warps 10 and 11; one K tile, by TMA, the two in turn, by
-          // copies each half of its rows.  Nobody may skip more than NSLOT units: a slot's barrier tells a phase
-          // only from the one before, and a warp knows that the use before last is over by its own last unit.
-          const bool halves = C::KT == 1 && k == 0 && !by_tma;
-          if (k < 0 ? warp != 8 : warp == 8 || (!halves && warp != 10 + (C::KT == 2 ? k : (j - j0) & 1))) continue;
+          // Who takes it: V warp 8; two K tiles of a block warps 10 and 11, one K tile these two in turn.  Nobody may
+          // skip more than NSLOT units: a slot's barrier tells a phase only from the one before, and a warp knows
+          // that the use before last is over by its own last unit.
+          if (warp != (k < 0 ? 8 : 10 + (C::KT == 2 ? k : (j - j0) & 1))) continue;
           const int st = unit % C::NSLOT;
           const uint32_t dst = ring0 + st * C::SLOT;
           const int head0 = head * MAPS + (k < 0 ? slice * C::DV / D : k);
           const int live = kv_end - j * kTcBlock;  // keys of the block that exist
-          // One lane for each box (TMA), each 16 tokens, or each of four times 32 tokens: where their rows are.
+          // One lane for each box, or for each of four times 32 tokens: where their rows are.
           int64_t row[4] = {-1, -1, -1, -1};
           unsigned bad[4] = {0, 0, 0, 0};
           int phys = p.num_blocks, off = 0;  // the block behind the last is out of the map: zeros
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (whole && i) break;
-            const int in = by_tma ? lane * bt : whole ? 16 * lane : 32 * i + lane;
+            const int in = whole ? lane * bt : 32 * i + lane;
             bool astray = false;
             if (in < kTcBlock && in < live) {
               const int token = j * kTcBlock + in, page = token / p.page;
@@ -651,18 +617,17 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             }
             bad[i] = __ballot_sync(kFull, astray);
           }
-          if (whole && bad[0]) {  // a bit a box or 16 tokens -> a bit a token
+          if (whole && bad[0]) {  // a bit a box -> a bit a token
             const unsigned pieces = bad[0];
-            const int each = by_tma ? bt : 16;
             for (int i = 0; i < 4; ++i) {
               bad[i] = 0;
-              for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / each)) & 1u) << e;
+              for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / bt)) & 1u) << e;
             }
           }
           if (!tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag)) break;
-          if (k == 0 && lane == 0 && !(halves && warp == 11))  // ahead of the block's scores
+          if (k == 0 && lane == 0)  // ahead of the block's scores
             *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
-          if (by_tma) {
+          if (whole) {
             const bool tail = k < 0 && live < kTcBlock && live % bt != 0;  // V rows behind the last key in its box
             const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
             if (lane == 0) mbar_arrive_expect_tx(bar, 128 * 2 * (k < 0 ? C::DV : D));
@@ -693,15 +658,11 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
               mbar_arrive(full0 + 8 * st);
             }
           } else {
-            constexpr int PARTS = C::KT == 1 ? 2 : 1;
-            const int part = PARTS == 2 ? warp - 10 : 0;
-            if (whole) tc_copy_pages<C::KH, D, PARTS>(dst, (const __half*)p.k, row[0], p.kv_st, p.kv_sh, live, part, lane);
-            else if (k < 0) tc_copy_rows<C::VC, D, 1>(dst, (const __half*)p.v, row, p.kv_sh, 0, lane);
-            else tc_copy_rows<C::KH, D, PARTS>(dst, (const __half*)p.k, row, p.kv_sh, part, lane);
+            if (k < 0) tc_copy_rows<C::VC, D>(dst, (const __half*)p.v, row, p.kv_sh, lane);
+            else tc_copy_rows<C::KH, D>(dst, (const __half*)p.k, row, p.kv_sh, lane);
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
-            __syncwarp();
-            if (!halves || lane < 16) mbar_arrive(full0 + 8 * st);  // 32 arrivals a unit
+            mbar_arrive(full0 + 8 * st);
           }
         }
         if (*abort_flag && issued >= 0) {  // boxes still in flight get a bounded chance to land
