@@ -176,7 +176,7 @@ int tc_run(const PdPrefillArgs* a, const PrefillParams& r, int sm_count) {
   memset(&mv, 0, sizeof(mv));
   tp.box_tokens = 16;  // the largest power of two up to a block that divides the page
   while (tp.box_tokens < kTcBlock && a->block_size % (2 * tp.box_tokens) == 0) tp.box_tokens *= 2;
-  if (a->kv_dtype <= PD_KV_BF16 && a->block_size % 16 == 0) {  // encoded for every call: nothing is kept by an address
+  if (a->block_size % 16 == 0) {  // encoded for every call: nothing is kept by an address
     if (!encode_page_box(a, a->k_cache, tp.box_tokens, &mk) || !encode_page_box(a, a->v_cache, tp.box_tokens, &mv))
       return PD_ERR_CUDA;
   }

@@ -65,7 +65,9 @@ struct TcCfg {
   static constexpr int SCALE_FLOATS = SCALED ? (KT + VH) * 128 : 0;  // of one block
   static constexpr int SCALE_RING = 8;                     // more blocks than the ring of tiles can be ahead of the softmax
   static constexpr int MISC = 1024 + (MAPS == 2 ? 2560 : 0);
-  static constexpr int FIXED = 1024 + 2 * QTILE + SCALE_RING * SCALE_FLOATS * 4 + MISC;
+  static constexpr int RAW = WIDEN ? 128 * (D > DV ? D : DV) : 0;      // one 8-bit tile as it comes
+  static constexpr int NRAW = 3;
+  static constexpr int FIXED = 1024 + 2 * QTILE + SCALE_RING * SCALE_FLOATS * 4 + NRAW * RAW + MISC;
   static constexpr int FIT = (kTcSmem - FIXED) / SLOT;
   static constexpr int NSLOT = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = FIXED + NSLOT * SLOT;
@@ -73,10 +75,11 @@ struct TcCfg {
   static constexpr int WARPS = WIDEN ? 16 : 12;
   // Registers.  A scheduler has a warp of each tile's softmax, one of the third group and, with 8-bit pages,
   // one that widens; what they hold adds up to the launch's 3 * 168 or 4 * 128.
-  static constexpr int REGS_SOFTMAX = WIDEN ? 176 : 200, REGS_THIRD = WIDEN ? 56 : 104, REGS_WIDEN = 104;
+  static constexpr int REGS_SOFTMAX = WIDEN ? 176 : 200, REGS_THIRD = WIDEN ? 80 : 104, REGS_WIDEN = 80;
   static_assert(WIDEN ? 2 * REGS_SOFTMAX + REGS_THIRD + REGS_WIDEN <= 4 * 128 : 2 * REGS_SOFTMAX + REGS_THIRD <= 3 * 168, "registers");
   static constexpr int THREADS = WARPS * 32;
-  static_assert(NSLOT >= (WIDEN ? 3 : 4) && SMEM <= kTcSmem, "shared memory; a loader's own units are at most four apart");
+  static constexpr int RING = WIDEN ? NRAW : NSLOT;        // what the loaders fill
+  static_assert(NSLOT >= (WIDEN ? 3 : 4) && NRAW >= KT + 1 && SMEM <= kTcSmem, "shared memory; how far a loader's units are apart");
 };
 
 struct TcParams {
@@ -260,17 +263,16 @@ __device__ __forceinline__ int64_t tc_place(const Params& p, int request, int to
     return kv_row_offset(p, id, token - page * p.page, 0);
   }
   if (p.status) atomicOr(p.status, PD_DEV_BAD_BLOCK);
-  atomicOr(mask, bits);
+  if (mask) atomicOr(mask, bits);
   return -1;
 }
 
-// The 16-byte pieces of an 8-bit tile that thread `me` of 128 takes: piece c of the rows r0, r0 + 128 / P, ..
-// `where` of lane l: tc_place of token 16 l of the block (whole pages of 16 tokens).  Bit i of the answer:
-// piece i exists.  All addresses first, then all loads, and nothing that uses one: the loads are to be in
-// flight together, until the pieces are widened (a use behind each load made a tile cost eight round trips).
+// The 16-byte pieces of an 8-bit tile that thread `me` of 128 takes, from pages of odd sizes: piece c of the rows
+// r0, r0 + 128 / P, ..  Bit i of the answer: piece i exists.  All addresses first, then all loads, and nothing
+// that uses one: they are to be in flight together.
 template <int P, int D, int PM>
-__device__ __forceinline__ unsigned tc_fetch(const Params& p, int request, int j, int h, const void* cache, bool whole, int64_t where,
-                                             int kv_end, unsigned* mask, int me, uint4 (&x)[PM]) {
+__device__ __forceinline__ unsigned tc_fetch(const Params& p, int request, int j, int h, const void* cache, int kv_end,
+                                             unsigned* mask, int me, uint4 (&x)[PM]) {
   const int c = me % P, r0 = me / P;
   const char* mine = (const char*)cache + (int64_t)(h + c * 16 / D) * p.kv_sh + c * 16 % D;
   const uint4* from[P];
@@ -278,19 +280,28 @@ __device__ __forceinline__ unsigned tc_fetch(const Params& p, int request, int j
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int r = r0 + i * (128 / P);
-    int64_t at;
-    if (whole) {
-      at = __shfl_sync(0xffffffffu, where, r / 16);
-      if (at >= 0) at = j * kTcBlock + r < kv_end ? at + (int64_t)(r & 15) * p.kv_st : -1;
-    } else {
-      int64_t unused;
-      at = tc_place(p, request, j * kTcBlock + r, kv_end, mask + r / 32, 1u << (r & 31), unused);
-    }
+    int64_t unused;
+    const int64_t at = tc_place(p, request, j * kTcBlock + r, kv_end, mask + r / 32, 1u << (r & 31), unused);
     live |= (at >= 0 ? 1u : 0u) << i;
     from[i] = reinterpret_cast<const uint4*>(mine + (at >= 0 ? at : 0));  // some row of the pool where there is none
   }
 #pragma unroll
   for (int i = 0; i < P; ++i) x[i] = __ldg(from[i]);
+  return live;
+}
+// The same pieces from a tile that has come by TMA; rows behind the last key (whatever their page holds) are left out.
+template <int P, int D, int PM>
+__device__ __forceinline__ unsigned tc_take(uint32_t raw, int keys, int me, uint4 (&x)[PM]) {
+  const int c = me % P, r0 = me / P;
+  unsigned live = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int r = r0 + i * (128 / P);
+    uint32_t w[4];
+    lds128(raw + (c * 16 / D) * (128 * D) + r * D + c * 16 % D, w);
+    x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    live |= (r < keys ? 1u : 0u) << i;
+  }
   return live;
 }
 
@@ -366,9 +377,11 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
+  // ring of tiles, Q, scales, 8-bit tiles, the rest
   const uint32_t ring0 = base, q0 = base + C::NSLOT * C::SLOT;
+  const uint32_t raw0 = q0 + 2 * C::QTILE + C::SCALE_RING * C::SCALE_FLOATS * 4;
   float* scales = reinterpret_cast<float*>(smem + C::NSLOT * C::SLOT + 2 * C::QTILE);
-  uint8_t* misc = smem + C::NSLOT * C::SLOT + 2 * C::QTILE + C::SCALE_RING * C::SCALE_FLOATS * 4;
+  uint8_t* misc = smem + C::NSLOT * C::SLOT + 2 * C::QTILE + C::SCALE_RING * C::SCALE_FLOATS * 4 + C::NRAW * C::RAW;
   unsigned* meta = reinterpret_cast<unsigned*>(misc);  // [block mod 16][4]: its tokens whose page is not in the pool
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 256);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc + 260);
@@ -376,7 +389,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   TcTile* tile_sh = reinterpret_cast<TcTile*>(misc + 272);
   const uint32_t bars = smem_u32(misc) + 320;
   const uint32_t full0 = bars, empty0 = bars + 64, s_full = bars + 128, o_done = bars + 144, q_full = bars + 160,
-                 drain_bar = bars + 168, tail_bar = bars + 208, p_full = bars + 176;  // p_full: [tile][half of the keys]
+                 drain_bar = bars + 168, tail_bar = bars + 208, raw_full = bars + 216, raw_empty = bars + 248, p_full = bars + 176;  // p_full: [tile][half of the keys]
   float* squares = reinterpret_cast<float*>(misc + 640);  // [tile][128] of this CTA's columns, then of the peer's
   float* weights = reinterpret_cast<float*>(misc + 640 + 2048);  // the norm's, of the slice
   static_assert(kTcMetaRing * 16 <= 256 && (MAPS == 1 ? 640 : 640 + 2048 + 512) <= C::MISC, "misc area");
@@ -411,13 +424,15 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     }
     mbar_init(q_full, 256);
     mbar_init(drain_bar, 1);
+    for (int s = 0; s < C::NRAW; ++s) {
+      mbar_init(raw_full + 8 * s, 32);
+      mbar_init(raw_empty + 8 * s, 128);
+    }
     mbar_init(tail_bar, 1);
     fence_barrier_init();
     fence_proxy_async();
-    if constexpr (!C::WIDEN) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&tm_k) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&tm_v) : "memory");
-    }
+    asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&tm_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((unsigned long long)&tm_v) : "memory");
   }
   __syncthreads();
   if (!*have_tile) return;  // the whole cluster has the same tile: nobody waits for this CTA
@@ -452,74 +467,56 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   const int kv_end = tc_limit(tile, last_row, p.group);  // keys from here on are zeros in shared memory
 
   // ================================ widening warps (8-bit pages) =======================================
-  // Four warps; a thread takes 16-byte pieces me, me + 128, .. of a tile's rows.  The pieces of the next unit
-  // are on their way while this one's are widened and stored, and the block ids of a block are fetched a
-  // block ahead (without that a tile cost two round trips to memory).
+  // Four warps; a thread takes the 16-byte pieces me, me + 128, .. of a tile's rows.  The tiles come by TMA (by
+  // plain loads they came at 5 bytes a cycle, half the time of a block); the scales, two bytes a token, are
+  // fetched a block ahead by the thread that owns the token.
   if (warp >= 12) {
     if constexpr (C::WIDEN) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_WIDEN));
       const int me = tid - 384;  // 0 .. 127
       constexpr int PK = D / 16, PV = C::DV / 16;        // 16-byte pieces of a K and of a V row = of a thread
       constexpr int PM = PK > PV ? PK : PV;
+      constexpr int NS = SCALED ? C::KT + C::VH : 1;
       const int nb = jend - j0;
       const int units = nb > 0 ? nb * (C::KT + 1) : 0;
-      const bool whole = p.page % 16 == 0;               // 16 tokens lie in one page
-      // lane l < 8 for tokens 16 l .. of block j
-      auto locate = [&](int j, int64_t& scale_at) -> int64_t {
-        scale_at = 0;
-        if (!whole || lane >= 8) return -1;
-        return tc_place(p, tile.request, j * kTcBlock + 16 * lane, kv_end, meta + 4 * (j & (kTcMetaRing - 1)) + lane / 2,
-                        0xffffu << (16 * (lane & 1)), scale_at);
-      };
-      auto fetch_unit = [&](int j, int k, int64_t where, int64_t scale_where, uint4 (&x)[PM], __half (&sc)[SCALED ? C::KT + C::VH : 1]) {
-        unsigned* mask = meta + 4 * (j & (kTcMetaRing - 1));
-        unsigned got;
-        if (k < 0) got = tc_fetch<PV, D, PM>(p, tile.request, j, head * MAPS + slice * C::DV / D, p.v, whole, where, kv_end, mask, me, x);
-        else got = tc_fetch<PK, D, PM>(p, tile.request, j, head * MAPS + k, p.k, whole, where, kv_end, mask, me, x);
+      const bool whole = p.page % 16 == 0;               // the loaders bring the tiles, and note pages outside the pool
+      // the scales of token `me` of block j, K's and V's: the softmax needs V's ahead of V itself
+      auto fetch_scales = [&](int j, __half (&sc)[NS]) {
         if constexpr (SCALED) {
-          // the block's scales, K's and V's, with its first K tile: the softmax needs them ahead of V itself
-          if (k == 0) {
-            int64_t at = __shfl_sync(kFull, scale_where, me / 16);
-            bool live = __shfl_sync(kFull, where, me / 16) >= 0 && j * kTcBlock + me < kv_end;
-            at += (int64_t)(me & 15) * p.sc_st;
-            if (!whole) live = tc_place(p, tile.request, j * kTcBlock + me, kv_end, mask + me / 32, 1u << (me & 31), at) >= 0;
-            at = (live ? at : 0) + head * MAPS;
+          int64_t at;
+          const bool live = j < jend && tc_place(p, tile.request, j * kTcBlock + me, kv_end, nullptr, 0, at) >= 0;
+          at = (live ? at : 0) + head * MAPS;
 #pragma unroll
-            for (int z = 0; z < C::KT; ++z) sc[z] = __ldg(p.k_scale + at + z);
+          for (int z = 0; z < C::KT; ++z) sc[z] = __ldg(p.k_scale + at + z);
 #pragma unroll
-            for (int z = 0; z < C::VH; ++z) sc[C::KT + z] = __ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0));
-            if (live) got |= 1u << 31;
-          }
+          for (int z = 0; z < C::VH; ++z) sc[C::KT + z] = __ldg(p.v_scale + at + (MAPS == 2 ? slice * C::DV / D + z : 0));
+          return live;
+        } else {
+          return true;
         }
-        return got;
       };
-      // where the tokens of block idj and of the one behind it lie
-      int64_t s_here, s_next;
-      int64_t here = locate(j0, s_here), next = locate(j0 + 1, s_next);
-      int idj = j0;
-      uint4 x[PM];
-      __half sc[SCALED ? C::KT + C::VH : 1];
-      unsigned live = units > 0 ? fetch_unit(j0, 0, here, s_here, x, sc) : 0;  // pieces of x, and bit 31: of sc
+      __half sc[NS];
+      bool sc_live = units > 0 && fetch_scales(j0, sc);
       bool ok = true;
       for (int unit = 0; unit < units && ok; ++unit) {
         int j, k;
         tc_unit<C::KT>(unit, j0, j, k);
-        uint4 nx[PM];
-        __half nsc[SCALED ? C::KT + C::VH : 1];
-        unsigned nlive = 0;
-        if (unit + 1 < units) {
-          int j2, k2;
-          tc_unit<C::KT>(unit + 1, j0, j2, k2);
-          // a block's V comes behind its K, the next block's K behind that: its tokens are located with this V
-          if (j2 > idj && k2 < 0) {
-            here = next;
-            s_here = s_next;
-            ++idj;
-            // the mask of a block read long ago, of one to be located far ahead
-            if (me < 4) meta[4 * ((idj + 1 + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;
-            next = locate(idj + 1, s_next);
-          }
-          nlive = fetch_unit(j2, k2, j2 > idj ? next : here, j2 > idj ? s_next : s_here, nx, nsc);
+        unsigned* mask = meta + 4 * (j & (kTcMetaRing - 1));
+        uint4 x[PM];
+        unsigned live;
+        if (whole) {
+          const int rs = unit % C::NRAW;
+          ok = tc_wait(raw_full + 8 * rs, (uint32_t)(unit / C::NRAW) & 1u, p.status, abort_flag);
+          if (!ok) break;
+          const uint32_t raw_tile = raw0 + rs * C::RAW;
+          live = k < 0 ? tc_take<PV, D, PM>(raw_tile, kv_end - j * kTcBlock, me, x)
+                       : tc_take<PK, D, PM>(raw_tile, kv_end - j * kTcBlock, me, x);
+          mbar_arrive(raw_empty + 8 * rs);
+        } else {
+          // the mask of a block read long ago, of one far ahead
+          if (k == 0 && me < 4) meta[4 * ((j + kTcMetaRing / 2) & (kTcMetaRing - 1)) + me] = 0;
+          live = k < 0 ? tc_fetch<PV, D, PM>(p, tile.request, j, head * MAPS + slice * C::DV / D, p.v, kv_end, mask, me, x)
+                       : tc_fetch<PK, D, PM>(p, tile.request, j, head * MAPS + k, p.k, kv_end, mask, me, x);
         }
         const int st = unit % C::NSLOT;
         const uint32_t dst = ring0 + st * C::SLOT;
@@ -553,29 +550,24 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
         if constexpr (SCALED) {
           if (k == 0) {
 #pragma unroll
-            for (int z = 0; z < C::KT + C::VH; ++z)
+            for (int z = 0; z < NS; ++z)
               scales[(j % C::SCALE_RING) * C::SCALE_FLOATS + z * 128 + me] =
-                  live >> 31 ? __half2float(sc[z]) * (z < C::KT ? 1.f : kBoost) : 0.f;
+                  sc_live ? __half2float(sc[z]) * (z < C::KT ? 1.f : kBoost) : 0.f;
           }
         }
         fence_proxy_async();
         mbar_arrive(full0 + 8 * st);
-#pragma unroll
-        for (int i = 0; i < PM; ++i) x[i] = nx[i];
-        live = nlive;
-        if constexpr (SCALED) {
-#pragma unroll
-          for (int z = 0; z < C::KT + C::VH; ++z) sc[z] = nsc[z];
-        }
+        if (k == 0) sc_live = fetch_scales(j + 1, sc);
       }
     }
   }
   // ================================ the third group: loaders and the matrix units' warp =================
   else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_THIRD));
-    // ================================ loaders (16-bit pages) =============================================
-    // V's tiles: warp 8; K's: warps 10 and 11.
-    if constexpr (!C::WIDEN) {
+    // ================================ loaders ==============================================================
+    // V's tiles: warp 8; K's: warps 10 and 11.  16-bit tiles go to the ring that the products read, 8-bit ones
+    // to the one that the widening warps read (which fetch pages of odd sizes themselves).
+    if (!C::WIDEN || p.page % 16 == 0) {
       if (warp != 9) {
         const int nb = jend - j0;
         const int units = nb > 0 ? nb * (C::KT + 1) : 0;
@@ -587,11 +579,12 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           int j, k;  // block; K tile number or -1: V
           tc_unit<C::KT>(unit, j0, j, k);
           // Who takes it: V warp 8; two K tiles of a block warps 10 and 11, one K tile these two in turn.  Nobody may
-          // skip more than NSLOT units: a slot's barrier tells a phase only from the one before, and a warp knows
-          // that the use before last is over by its own last unit.
-          if (warp != (k < 0 ? 8 : 10 + (C::KT == 2 ? k : (j - j0) & 1))) continue;
-          const int st = unit % C::NSLOT;
-          const uint32_t dst = ring0 + st * C::SLOT;
+          // skip more units than the ring has slots: a slot's barrier tells a phase only from the one before, and
+          // a warp knows that the use before last is over by its own last unit.
+          if (warp != (k < 0 ? 8 : 10 + (C::KT == 2 ? k : C::WIDEN ? 0 : (j - j0) & 1))) continue;
+          const int st = unit % C::RING;
+          const uint32_t dst = C::WIDEN ? raw0 + st * C::RAW : ring0 + st * C::SLOT;
+          const uint32_t is_full = (C::WIDEN ? raw_full : full0) + 8 * st, is_empty = (C::WIDEN ? raw_empty : empty0) + 8 * st;
           const int head0 = head * MAPS + (k < 0 ? slice * C::DV / D : k);
           const int live = kv_end - j * kTcBlock;  // keys of the block that exist
           // One lane for each box, or for each of four times 32 tokens: where their rows are.
@@ -624,12 +617,26 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
               for (int e = 0; e < 32; ++e) bad[i] |= ((pieces >> ((32 * i + e) / bt)) & 1u) << e;
             }
           }
-          if (!tc_wait(empty0 + 8 * st, ((uint32_t)(unit / C::NSLOT) & 1u) ^ 1u, p.status, abort_flag)) break;
+          if (!tc_wait(is_empty, ((uint32_t)(unit / C::RING) & 1u) ^ 1u, p.status, abort_flag)) break;
           if (k == 0 && lane == 0)  // ahead of the block's scores
             *reinterpret_cast<uint4*>(meta + 4 * (j & (kTcMetaRing - 1))) = make_uint4(bad[0], bad[1], bad[2], bad[3]);
-          if (whole) {
+          if constexpr (C::WIDEN) {
+            if (lane == 0) mbar_arrive_expect_tx(is_full, 128 * (k < 0 ? C::DV : D));
+            else mbar_arrive(is_full);
+            __syncwarp();
+            issued = unit;
+            if (lane < boxes) {  // whole rows of a head: planes of 128 rows of D bytes
+              if (k >= 0) {
+                tma_load_4d(dst + lane * bt * D, &tm_k, is_full, 0, off, head0, phys);
+              } else {
+#pragma unroll
+                for (int z = 0; z < C::VH; ++z) tma_load_4d(dst + z * (128 * D) + lane * bt * D, &tm_v, is_full, 0, off, head0 + z, phys);
+              }
+            }
+            __syncwarp();
+          } else if (whole) {
             const bool tail = k < 0 && live < kTcBlock && live % bt != 0;  // V rows behind the last key in its box
-            const uint32_t bar = tail ? tail_bar : full0 + 8 * st;
+            const uint32_t bar = tail ? tail_bar : is_full;
             if (lane == 0) mbar_arrive_expect_tx(bar, 128 * 2 * (k < 0 ? C::DV : D));
             if (lane > 0 && !tail) mbar_arrive(bar);
             __syncwarp();
@@ -655,19 +662,19 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
                 sts128(dst + tc_row(r, c) + (i & 7) * 16, make_uint4(0, 0, 0, 0));
               }
               fence_proxy_async();
-              mbar_arrive(full0 + 8 * st);
+              mbar_arrive(is_full);
             }
           } else {
             if (k < 0) tc_copy_rows<C::VC, D>(dst, (const __half*)p.v, row, p.kv_sh, lane);
             else tc_copy_rows<C::KH, D>(dst, (const __half*)p.k, row, p.kv_sh, lane);
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
-            mbar_arrive(full0 + 8 * st);
+            mbar_arrive(is_full);
           }
         }
         if (*abort_flag && issued >= 0) {  // boxes still in flight get a bounded chance to land
-          for (int u = issued; u >= 0 && u > issued - C::NSLOT; --u)
-            tc_drain(full0 + 8 * (u % C::NSLOT), (uint32_t)(u / C::NSLOT) & 1u);
+          for (int u = issued; u >= 0 && u > issued - C::RING; --u)
+            tc_drain((C::WIDEN ? raw_full : full0) + 8 * (u % C::RING), (uint32_t)(u / C::RING) & 1u);
           if (tail_used) tc_drain(tail_bar, 0);
         }
       }

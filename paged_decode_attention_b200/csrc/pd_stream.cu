@@ -234,15 +234,18 @@ static bool encode_tensor_map_in_place(const MapKey& k, CUtensorMap* out) {
 bool encode_page_box(const PdPrefillArgs* a, const void* cache, int box_tokens, CUtensorMap* out) {
   EncodeFn enc = encode_fn();
   if (!enc) return false;
+  const bool wide = is_16bit(a->kv_dtype);
+  const int eb = wide ? 2 : 1;
   const cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->block_size, (cuuint64_t)a->num_kv_heads,
                               (cuuint64_t)a->num_blocks};
-  const cuuint64_t strides[3] = {(cuuint64_t)a->kv_stride_token * 2, (cuuint64_t)a->kv_stride_head * 2,
-                                 (cuuint64_t)a->kv_stride_block * 2};
-  const cuuint32_t box[4] = {64u, (cuuint32_t)box_tokens, 1u, 1u};
+  const cuuint64_t strides[3] = {(cuuint64_t)a->kv_stride_token * eb, (cuuint64_t)a->kv_stride_head * eb,
+                                 (cuuint64_t)a->kv_stride_block * eb};
+  const cuuint32_t box[4] = {wide ? 64u : (cuuint32_t)a->head_dim, (cuuint32_t)box_tokens, 1u, 1u};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return enc(out, a->kv_dtype == PD_KV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-             const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return enc(out, a->kv_dtype == PD_KV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+             4, const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // The same through a small cache keyed by everything the encoding depends on.

@@ -30,8 +30,8 @@ int diff_stream_supports(const PdPrefillArgs* a);
 uint64_t diff_stream_workspace_bytes(const PdPrefillArgs* a, int sm_count);
 int diff_stream_run(const PdPrefillArgs* a, int sm_count);
 
-// Tensor map of one 16-bit cache tensor with boxes of 64 elements, `box_tokens` tokens and one head, in the
-// 128-byte swizzle.
+// Tensor map of one cache tensor with boxes of `box_tokens` tokens of one head: 64 columns in the 128-byte
+// swizzle (16-bit pages), whole rows as they are (8-bit).
 bool encode_page_box(const PdPrefillArgs* a, const void* cache, int box_tokens, CUtensorMap* out);
 
 // Defined in pd_api.cu: argument checks that need no device, the device-side parameter block,
