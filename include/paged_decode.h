@@ -351,7 +351,10 @@ PD_API int pd_cache_write(const PdCacheWriteArgs* args);
  * rounded to q's type for the product with V by the kernels that use the matrix units.
  *
  * Keys and values of 8-bit pages are stored * scale, unrounded.  A block id outside the pool sets
- * PD_DEV_BAD_BLOCK and its tokens are left out. */
+ * PD_DEV_BAD_BLOCK and its tokens are left out.  Nothing behind a request's last token is used, whatever
+ * is stored there; the values of its own tokens have to be finite (one that is not may reach rows in
+ * front of its token, because rows are multiplied by blocks: zero times infinity is NaN).  With 8-bit
+ * pages on the matrix units a value scale is below 255. */
 typedef struct PdPrefillArgs {
   const void* q;   /* io_dtype, head_dim contiguous; strides: row, query head (maps = 2: query pair), map */
   void* out;       /* io_dtype, [rows, num_q_heads, head_dim], or [rows, num_q_heads / 2, 2 * head_dim] */
@@ -376,7 +379,7 @@ typedef struct PdPrefillArgs {
   int64_t lam_stride_t, lam_stride_h;
   float lam_value;
   const float* norm_weight;    /* [2 * head_dim] dense, or NULL: ones */
-  float eps, out_scale;
+  float eps, out_scale;        /* eps > 0 */
   int32_t norm;                /* 0: no norm */
   int32_t kernel;              /* PD_KERNEL_*: STREAM is the one on the matrix units */
   int32_t sm_count;            /* 0 = query the current device */

@@ -24,6 +24,7 @@ static int validate_prefill(const PdPrefillArgs* a) {
   if (a->io_dtype != PD_IO_F16 && a->io_dtype != PD_IO_BF16) return PD_ERR_INVALID_ARG;
   if (a->kernel < PD_KERNEL_AUTO || a->kernel > PD_KERNEL_STREAM) return PD_ERR_INVALID_ARG;
   if (a->max_seq_len < 0 || a->sm_count < 0) return PD_ERR_INVALID_ARG;
+  if (a->maps == 2 && a->norm && !(a->eps > 0.f)) return PD_ERR_INVALID_ARG;  // a row without keys is all zeros
   if ((a->k_scale == nullptr) != (a->v_scale == nullptr)) return PD_ERR_INVALID_ARG;
   if (a->kv_dtype == PD_KV_I8 && !a->k_scale) return PD_ERR_INVALID_ARG;
   if (a->kv_dtype <= PD_KV_BF16 && a->k_scale) return PD_ERR_INVALID_ARG;

@@ -101,7 +101,7 @@ constexpr int kTcMaxSplits = 64;
 constexpr int kTcLong = 16;
 
 struct TcPlan {
-  int tiles, heads, splits;
+  int tiles, heads, splits, target;
   int64_t grid;
   uint64_t lse_off, bytes;
 };
@@ -112,17 +112,18 @@ static TcPlan tc_plan(const PdPrefillArgs* a, int sm_count) {
   const int group = a->num_q_heads / a->num_kv_heads;
   t.tiles = (int)((int64_t)a->num_rows * group / s.rows + a->batch);
   t.heads = a->num_kv_heads / a->maps;
-  // Split the keys where the tiles alone would leave SMs idle.  Up to half a wave of tiles: as many splits
-  // as fill one wave, of kTcLeast blocks and more.  Up to two waves: three waves of pieces of at least
-  // kTcLong blocks, because contexts of a batch differ and the last tile to end is a long one; shorter pieces
-  // cost more in starts and in the join than they even out (2048 tokens of 32/8 heads, 264 tiles: 56 us, in
-  // two pieces 100 us).  Beyond, the order of the tiles evens it out.
+  // Split the keys where the tiles alone would leave SMs idle; the kernel cuts them into pieces of equal length.
+  // Up to half a wave of tiles: pieces for one wave, of kTcLeast blocks and more, with room for twice as many
+  // pieces of a context as of the mean one.  Up to two waves: pieces for three waves, of at least kTcLong blocks,
+  // because contexts of a batch differ and the last tile to end is a long one; shorter pieces cost more in
+  // starts and in the join than they even out (2048 tokens of 32/8 heads, 264 tiles: 56 us, in two pieces
+  // 100 us).  Beyond, the order of the tiles evens it out.
   int64_t bound = (int64_t)a->max_blocks_per_seq * a->block_size;
   if (a->max_seq_len > 0 && a->max_seq_len < bound) bound = a->max_seq_len;
   const int64_t ctas = (int64_t)t.tiles * t.heads * s.slices;
   int64_t n = 1;
   if (ctas * 2 <= sm_count) {
-    n = sm_count / (ctas > 0 ? ctas : 1);
+    n = 2 * sm_count / (ctas > 0 ? ctas : 1);
     if (n > bound / kTcBlock / kTcLeast) n = bound / kTcBlock / kTcLeast;
   } else if (ctas < 2 * sm_count) {
     n = (3 * sm_count + ctas - 1) / ctas;
@@ -130,6 +131,7 @@ static TcPlan tc_plan(const PdPrefillArgs* a, int sm_count) {
   }
   if (n > kTcMaxSplits) n = kTcMaxSplits;
   t.splits = n < 1 ? 1 : (int)n;
+  t.target = ctas * 2 <= sm_count ? sm_count - (int)ctas : 3 * sm_count;  // one wave: every tile may end with a short piece
   t.grid = ctas * t.splits;
   t.lse_off = t.bytes = 0;
   if (t.splits > 1) {
@@ -169,6 +171,7 @@ int tc_run(const PdPrefillArgs* a, const PrefillParams& r, int sm_count) {
   tp.tiles = t.tiles;
   tp.heads = t.heads;
   tp.splits = t.splits;
+  tp.target = t.target;
   tp.part_o = t.bytes ? (float*)a->workspace : nullptr;
   tp.part_lse = t.bytes ? (float*)((char*)a->workspace + t.lse_off) : nullptr;
   CUtensorMap mk, mv;

@@ -51,7 +51,7 @@ constexpr int kTcSmem = 227 * 1024;
 
 template <int KV, int D, int MAPS, bool SCALED>
 struct TcCfg {
-  static constexpr bool WIDEN = !is_16bit(KV);             // 8-bit pages: converting warps instead of TMA
+  static constexpr bool WIDEN = !is_16bit(KV);             // 8-bit pages: four warps widen the tiles
   static constexpr bool BF16 = KV == PD_KV_BF16;
   static constexpr int DV = MAPS == 2 ? 128 : D;           // columns of V in one CTA
   static constexpr int SLICES = MAPS * D / DV;             // CTAs that share V's columns
@@ -86,6 +86,7 @@ struct TcParams {
   PrefillParams a;
   int32_t tiles, heads, splits;  // grid: splits x tiles x heads (x slices)
   int32_t box_tokens;            // tokens of one TMA box
+  int32_t target;                // CTAs to share the key blocks out over
   float* part_o;                 // splits > 1: [split][row][head, map][columns of V in all], log-sum-exps
   float* part_lse;
 };
@@ -217,6 +218,12 @@ __device__ __forceinline__ void tc_add2(float& x, float& y, float f, float g) { 
       : "+f"(x), "+f"(y)
       : "f"(f), "f"(g));
 }
+__device__ __forceinline__ void tc_mul2(float& x, float& y, float f, float g) {  // (x, y) = (x * f, y * g)
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(f), "f"(g));
+}
 __device__ __forceinline__ float tc_max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -305,6 +312,27 @@ __device__ __forceinline__ unsigned tc_take(uint32_t raw, int keys, int me, uint
   return live;
 }
 
+// A warp's 32 result rows of CH 16-byte chunks, from a thread a row to whole rows at a time: the chunks go through
+// 32 * CH * 16 bytes of shared memory (`area`), neighbouring lanes then store neighbouring chunks of a row.
+// (Straight from the threads a store touched 32 rows.)  `off` of lane l: where row l begins in out, -1: nowhere.
+template <int CH>
+__device__ __forceinline__ void tc_put_chunk(uint32_t area, int lane, int c, const uint4& y) {
+  sts128(area + lane * (CH * 16) + ((c ^ (lane & 7)) << 4), y);
+}
+template <int CH>
+__device__ __forceinline__ void tc_store_rows(uint32_t area, int lane, __half* out, int64_t off) {
+  __syncwarp();
+  const int c = lane % CH;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = i * (32 / CH) + lane / CH;
+    uint32_t w[4];
+    lds128(area + r * (CH * 16) + ((c ^ (r & 7)) << 4), w);
+    const int64_t at = __shfl_sync(0xffffffffu, off, r);
+    if (at >= 0) *reinterpret_cast<uint4*>(out + at + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // What a CTA works on.
 struct TcTile {
   int request, row0, count;  // first packed row (within the request) and packed rows, at most ROWS
@@ -386,6 +414,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 256);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(misc + 260);
   volatile int* have_tile = reinterpret_cast<volatile int*>(misc + 264);
+  volatile int* share = reinterpret_cast<volatile int*>(misc + 268);  // key blocks of a piece
   TcTile* tile_sh = reinterpret_cast<TcTile*>(misc + 272);
   const uint32_t bars = smem_u32(misc) + 320;
   const uint32_t full0 = bars, empty0 = bars + 64, s_full = bars + 128, o_done = bars + 144, q_full = bars + 160,
@@ -410,6 +439,22 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       if (ok) *tile_sh = t;
       *abort_flag = 0;
     }
+  }
+  // With splits: the key blocks of all tiles shared out evenly over the CTAs that there are SMs for, so that a
+  // long context is cut into more pieces than a short one (an even cut of each, nine pieces of contexts of
+  // 16 to 32 k: the longest pieces were half as long again as the mean).
+  if (warp == 1 && tp.splits > 1) {
+    long long sum = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+      const int tokens = __ldg(a.starts + b + 1) - __ldg(a.starts + b), len = __ldg(p.seq_lens + b);
+      if (tokens > 0 && len > 0) {
+        const long long tiles = ((long long)tokens * p.group + C::ROWS - 1) / C::ROWS;
+        sum += tiles * ((min((long long)len, (long long)p.max_blocks * p.page) + kTcBlock - 1) / kTcBlock);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (lane == 0) *share = (int)min((sum * tp.heads * C::SLICES + tp.target - 1) / tp.target, (long long)INT32_MAX);
   }
   if (warp == 8 && lane == 0) {
     for (int s = 0; s < C::NSLOT; ++s) {
@@ -454,7 +499,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
   int rows_of[2], begin[2], end[2];  // rows, first and last + 1 key block
   const int last_row = tile.row0 + tile.count - 1;
   const int blocks = (tc_limit(tile, last_row, p.group) + kTcBlock - 1) / kTcBlock;  // of the longest row
-  const int chunk = tp.splits > 1 ? max((blocks + tp.splits - 1) / tp.splits, kTcLeast) : blocks;
+  int chunk = blocks;
+  if (tp.splits > 1) chunk = max(max((blocks + tp.splits - 1) / tp.splits, *share), kTcLeast);
   const int j0 = min(split * chunk, blocks), j1 = min(j0 + chunk, blocks);
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -850,10 +896,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 f = *reinterpret_cast<const float4*>(ks + c0 + c);
-            x[c] *= f.x;
-            x[c + 1] *= f.y;
-            x[c + 2] *= f.z;
-            x[c + 3] *= f.w;
+            tc_mul2(x[c], x[c + 1], f.x, f.y);
+            tc_mul2(x[c + 2], x[c + 3], f.z, f.w);
           }
         }
         if (masked) {
@@ -904,7 +948,7 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           tc_fma2(y[c], y[c + 1], p.scale_log2, -from);
           y[c] = fast_exp2(y[c]);
           y[c + 1] = fast_exp2(y[c + 1]);
-          tc_add2(sum[c & 2], sum[(c & 2) + 1], y[c], y[c + 1]);
+          if constexpr (SCALED || MAPS == 1) tc_add2(sum[c & 2], sum[(c & 2) + 1], y[c], y[c + 1]);
         }
         uint32_t pk[16];
 #pragma unroll
@@ -912,13 +956,20 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           if constexpr (SCALED) {
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(vs + z * 128 + c0 + c);
-              pk[c / 2] = tc_pack<C::BF16>(y[c] * f.x, y[c + 1] * f.y);
-              pk[c / 2 + 1] = tc_pack<C::BF16>(y[c + 2] * f.z, y[c + 3] * f.w);
+              float4 f = *reinterpret_cast<const float4*>(vs + z * 128 + c0 + c);
+              tc_mul2(f.x, f.y, y[c], y[c + 1]);
+              tc_mul2(f.z, f.w, y[c + 2], y[c + 3]);
+              pk[c / 2] = tc_pack<C::BF16>(f.x, f.y);
+              pk[c / 2 + 1] = tc_pack<C::BF16>(f.z, f.w);
             }
           } else {
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) pk[c / 2] = tc_pack<C::BF16>(y[c], y[c + 1]);
+            for (int c = 0; c < 32; c += 2) {
+              pk[c / 2] = tc_pack<C::BF16>(y[c], y[c + 1]);
+              // For a pair l is the sum of what the product with V reads, the rounded probabilities: what their
+              // roundings have in common then cancels in O / l, which the difference of the two maps needs.
+              if constexpr (MAPS == 2) add_pair<C::BF16>(sum[c & 2], sum[(c & 2) + 1], pk[c / 2]);
+            }
           }
           // columns below 16 (or 32) * (c0 / 32 + 1) hold scores that have been read
           tc_st16(s_at + (C::NP == 1 ? c0 / 2 : c0 + 16 * z), pk);
@@ -943,6 +994,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     const int tok = pr / p.group, g = pr - tok * p.group;
     const int64_t row = tile.first_token + tok;
     const int hq = head * p.group + g;  // query head, or pair
+    // this warp's part of its tile's Q, which has been read: the results pass through it
+    const uint32_t area = q0 + t * C::QTILE + (warp & 3) * (C::QTILE / 4);
     if (tp.splits > 1) {
       const int64_t at = (((int64_t)split * a.rows + row) * (p.hq / MAPS) + hq) * MAPS + (MAPS == 2 ? t : 0);
 #pragma unroll 1
@@ -967,22 +1020,20 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
           tc_ld32(o_at + c0, o);
           tc_wait_ld();
         }
-        if (live && ok) {
-          uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh + c0);
-          const bool some = any && inv != 0.f;
+        const bool some = any && inv != 0.f;
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {
-            uint4 y = make_uint4(0, 0, 0, 0);
-            if (some) {
-              y.x = tc_pack<C::BF16>(o[c] * inv, o[c + 1] * inv);
-              y.y = tc_pack<C::BF16>(o[c + 2] * inv, o[c + 3] * inv);
-              y.z = tc_pack<C::BF16>(o[c + 4] * inv, o[c + 5] * inv);
-              y.w = tc_pack<C::BF16>(o[c + 6] * inv, o[c + 7] * inv);
-            }
-            dst[c / 8] = y;
+        for (int c = 0; c < 32; c += 8) {
+          uint4 y = make_uint4(0, 0, 0, 0);
+          if (some) {
+            y.x = tc_pack<C::BF16>(o[c] * inv, o[c + 1] * inv);
+            y.y = tc_pack<C::BF16>(o[c + 2] * inv, o[c + 3] * inv);
+            y.z = tc_pack<C::BF16>(o[c + 4] * inv, o[c + 5] * inv);
+            y.w = tc_pack<C::BF16>(o[c + 6] * inv, o[c + 7] * inv);
           }
+          tc_put_chunk<D / 8>(area, lane, (c0 + c) / 8, y);
         }
       }
+      tc_store_rows<D / 8>(area, lane, (__half*)p.out, live && ok ? row * p.o_sb + (int64_t)hq * p.o_sh : -1);
     } else {
       // A row's two maps are in two threads.  Through the ring (every tile in it has been read) the first map's
       // thread gets the second's columns 0..63 and gives its own 64..127, a column of 128 rows at a time:
@@ -1024,22 +1075,23 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       } else {
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      if (live && ok) {
+      {
         float total = squares[me] + squares[128 + me];
         if constexpr (C::SLICES == 2) total += squares[256 + me] + squares[384 + me];
         float factor = a.out_scale;
         if (a.norm) factor *= rsqrtf(total * (1.f / (MAPS * D)) + a.eps);
         const int col = slice * C::DV + t * 64;
-        uint4* dst = reinterpret_cast<uint4*>((__half*)p.out + row * p.o_sb + (int64_t)hq * p.o_sh + col);
         const float* wt = weights + t * 64;
 #pragma unroll
         for (int c = 0; c < 64; c += 8) {
           const float4 w0 = *reinterpret_cast<const float4*>(wt + c), w1 = *reinterpret_cast<const float4*>(wt + c + 4);
-          dst[c / 8] = make_uint4(tc_pack<C::BF16>(x[c] * factor * w0.x, x[c + 1] * factor * w0.y),
-                                  tc_pack<C::BF16>(x[c + 2] * factor * w0.z, x[c + 3] * factor * w0.w),
-                                  tc_pack<C::BF16>(x[c + 4] * factor * w1.x, x[c + 5] * factor * w1.y),
-                                  tc_pack<C::BF16>(x[c + 6] * factor * w1.z, x[c + 7] * factor * w1.w));
+          tc_put_chunk<8>(area, lane, c / 8,
+                          make_uint4(tc_pack<C::BF16>(x[c] * factor * w0.x, x[c + 1] * factor * w0.y),
+                                     tc_pack<C::BF16>(x[c + 2] * factor * w0.z, x[c + 3] * factor * w0.w),
+                                     tc_pack<C::BF16>(x[c + 4] * factor * w1.x, x[c + 5] * factor * w1.y),
+                                     tc_pack<C::BF16>(x[c + 6] * factor * w1.z, x[c + 7] * factor * w1.w)));
         }
+        tc_store_rows<8>(area, lane, (__half*)p.out, live && ok ? row * p.o_sb + (int64_t)hq * p.o_sh + col : -1);
       }
     }
   }

@@ -295,6 +295,16 @@ __device__ __forceinline__ uint32_t pack_io2(float lo, float hi) {
     return pack_half2(lo, hi);
   }
 }
+// x += the lower, y += the upper of a packed 16-bit pair, in 32 bits.
+template <bool BF16>
+__device__ __forceinline__ void add_pair(float& x, float& y, uint32_t pair) {
+  if constexpr (BF16)
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.bf16 %0, a, %0;\n\tadd.rn.f32.bf16 %1, b, %1;\n\t}"
+        : "+f"(x), "+f"(y) : "r"(pair));
+  else
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.f16 %0, a, %0;\n\tadd.rn.f32.f16 %1, b, %1;\n\t}"
+        : "+f"(x), "+f"(y) : "r"(pair));
+}
 template <int KV>
 __device__ __forceinline__ void store_io(void* row, int col, float x) {
   if constexpr (KV == PD_KV_BF16) ((__nv_bfloat16*)row)[col] = __float2bfloat16_rn(x);
@@ -377,7 +387,7 @@ __device__ __forceinline__ void consume_tile(
     const float scale_log2, const int lane,
     const uint32_t (&qb)[StreamCfg<KV, D, HB, SCALED>::KSTEPS][NG][2], const float (&qstep)[NG][2],
     float (&m)[NG][2], float (&l)[NG][2], float (&o)[MAPS * StreamCfg<KV, D, HB, SCALED>::MT][NG][4],
-    float (&psum)[SCALED ? MAPS : 1][NG][4], const int second = 0) {
+    float (&psum)[NG][4], const int second = 0) {
   using C = StreamCfg<KV, D, HB, SCALED>;
   constexpr unsigned kFull = 0xffffffffu;
   const int gq = lane >> 2, tq = lane & 3;
@@ -555,15 +565,23 @@ __device__ __forceinline__ void consume_tile(
     for (int u = 0; u < NT; ++u) {
       const float p0 = fast_exp2(x[u][0] - mn0), p1 = fast_exp2(x[u][1] - mn1);
       const float p2 = fast_exp2(x[u][2] - mn0), p3 = fast_exp2(x[u][3] - mn1);
-      sum0 += p0 + p2;
-      sum1 += p1 + p3;
+      if constexpr (MAPS == 1 || SCALED) {
+        sum0 += p0 + p2;
+        sum1 += p1 + p3;
+      }
       // (token g | g+8, heads 2t, 2t+1) -> (tokens 2t, 2t+1 | 2t+8, 2t+9, head g)
 #pragma unroll
       for (int z = 0; z < PV; ++z) {
-        pb[z][u][ng][0] =
-            movmatrix_trans(SCALED ? pack_io2<KV>(p0 * vs[z][u][0], p1 * vs[z][u][0]) : pack_io2<KV>(p0, p1));
-        pb[z][u][ng][1] =
-            movmatrix_trans(SCALED ? pack_io2<KV>(p2 * vs[z][u][1], p3 * vs[z][u][1]) : pack_io2<KV>(p2, p3));
+        const uint32_t lo = SCALED ? pack_io2<KV>(p0 * vs[z][u][0], p1 * vs[z][u][0]) : pack_io2<KV>(p0, p1);
+        const uint32_t hi = SCALED ? pack_io2<KV>(p2 * vs[z][u][1], p3 * vs[z][u][1]) : pack_io2<KV>(p2, p3);
+        if constexpr (MAPS == 2 && !SCALED) {
+          // the sum of the rounded probabilities, as the product reads them: what their roundings have in
+          // common cancels in O / l, which the difference of the two maps needs
+          add_pair<KV == PD_KV_BF16>(sum0, sum1, lo);
+          add_pair<KV == PD_KV_BF16>(sum0, sum1, hi);
+        }
+        pb[z][u][ng][0] = movmatrix_trans(lo);
+        pb[z][u][ng][1] = movmatrix_trans(hi);
       }
     }
     l[ng][0] = l[ng][0] * alpha[ng][0] + sum0;
@@ -581,16 +599,13 @@ __device__ __forceinline__ void consume_tile(
         o[mt][ng][3] *= alpha[ng][1];
       }
     }
-    if constexpr (KV == PD_KV_I8) {
+    if constexpr (KV == PD_KV_I8 && MAPS == 1) {
 #pragma unroll
-      for (int z = 0; z < PV; ++z) {
-#pragma unroll
-        for (int ng = 0; ng < NG; ++ng) {
-          psum[z][ng][0] *= alpha[ng][0];
-          psum[z][ng][1] *= alpha[ng][1];
-          psum[z][ng][2] *= alpha[ng][0];
-          psum[z][ng][3] *= alpha[ng][1];
-        }
+      for (int ng = 0; ng < NG; ++ng) {
+        psum[ng][0] *= alpha[ng][0];
+        psum[ng][1] *= alpha[ng][1];
+        psum[ng][2] *= alpha[ng][0];
+        psum[ng][3] *= alpha[ng][1];
       }
     }
   }
@@ -661,8 +676,10 @@ __device__ __forceinline__ void consume_tile(
           for (int h = 0; h < 2; ++h) {
             const int mt = c * (C::PITCH / 16) + 2 * i + h;
             uint32_t a[4];
-            if constexpr (KV == PD_KV_I8) {
-              // int8 values enter as 1152 + x (one prmt each); the surplus is taken out below
+            if constexpr (KV == PD_KV_I8 && MAPS == 1) {
+              // int8 values enter as 1152 + x (one prmt each); the surplus is taken out below.  (Not for a
+              // pair: the surplus is hundreds of times the result, and the difference of two maps would show
+              // what 32-bit accumulators lose on it - 6e-4 of the result, 3e-4 without.)
               a[0] = cvt_pair_biased(e01, h != 0);
               a[1] = cvt_pair_biased(o01, h != 0);
               a[2] = cvt_pair_biased(e23, h != 0);
@@ -686,19 +703,16 @@ __device__ __forceinline__ void consume_tile(
       }
     }
   }
-  if constexpr (KV == PD_KV_I8) {
+  if constexpr (KV == PD_KV_I8 && MAPS == 1) {
     // Every int8 value entered as 1152 + x.  One more mma with an all-ones A adds, in every row,
     // the sum over this call's tokens of P^T exactly as the tensor core read it to the running
     // column sums; they are rescaled with the accumulators, and 1152 times them leaves every
     // accumulator once, when the segment ends (no multiply-add per accumulator and tile).
     const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
 #pragma unroll
-    for (int z = 0; z < PV; ++z) {
+    for (int ng = 0; ng < NG; ++ng) {
 #pragma unroll
-      for (int ng = 0; ng < NG; ++ng) {
-#pragma unroll
-        for (int u = 0; u < NT; ++u) mma_kv<KV>(psum[z][ng], ones, pb[z][u][ng][0], pb[z][u][ng][1]);
-      }
+      for (int u = 0; u < NT; ++u) mma_kv<KV>(psum[ng], ones, pb[0][u][ng][0], pb[0][u][ng][1]);
     }
   }
 }
@@ -1399,12 +1413,9 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     for (int mt = 0; mt < MAPS * C::MT; ++mt)
 #pragma unroll
       for (int ng = 0; ng < NG; ++ng) o[mt][ng][0] = o[mt][ng][1] = o[mt][ng][2] = o[mt][ng][3] = 0.f;
-    constexpr int PV = SCALED ? MAPS : 1;
-    float psum[PV][NG][4];  // int8 pages: running column sums of P^T (see consume_tile)
+    float psum[NG][4];  // int8 pages: running column sums of P^T (see consume_tile)
 #pragma unroll
-    for (int z = 0; z < PV; ++z)
-#pragma unroll
-      for (int ng = 0; ng < NG; ++ng) psum[z][ng][0] = psum[z][ng][1] = psum[z][ng][2] = psum[z][ng][3] = 0.f;
+    for (int ng = 0; ng < NG; ++ng) psum[ng][0] = psum[ng][1] = psum[ng][2] = psum[ng][3] = 0.f;
 
     // 8-bit tiles with a deep ring (five stages or more) are taken two at a time: one softmax
     // step per 32 tokens and two independent score chains per warp.  With fewer stages the
@@ -1472,15 +1483,14 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     if (aborted) break;
 
     // ---- segment epilogue: the thread owns heads 2t, 2t+1 (+8 per n-tile) -----------------------
-    if constexpr (KV == PD_KV_I8) {
+    if constexpr (KV == PD_KV_I8 && MAPS == 1) {
       // the surplus of the biased int8 values: 1152 times the column sums of P^T, rows alike
 #pragma unroll
-      for (int mt = 0; mt < MAPS * C::MT; ++mt) {
+      for (int mt = 0; mt < C::MT; ++mt) {
 #pragma unroll
         for (int ng = 0; ng < NG; ++ng) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            o[mt][ng][r] = fmaf(-1152.f, psum[SCALED ? mt / C::MT : 0][ng][r], o[mt][ng][r]);
+          for (int r = 0; r < 4; ++r) o[mt][ng][r] = fmaf(-1152.f, psum[ng][r], o[mt][ng][r]);
         }
       }
     }

@@ -9,7 +9,10 @@ They read the cache that ``paged_decode`` reads, after ``cache_write`` has store
 ``kernel="auto"`` takes the kernels on the matrix units where they serve the request (head_dim 64
 and 128, q of the cache's own 16-bit type or fp16 with 8-bit pages, 16-byte aligned rows; single tokens:
 pages of a multiple of 16 tokens up to 256, groups of up to 16 heads) and a general kernel on the CUDA cores everywhere else.  There
-is no CPU or PyTorch fallback.
+is no CPU or PyTorch fallback and no autograd.
+
+What lies behind a request's last token in its pages is never used.  The values of its own tokens
+have to be finite: one that is not may reach query rows in front of it.
 """
 
 from __future__ import annotations
@@ -95,6 +98,10 @@ def build_prefill_args(q: torch.Tensor, cache: PagedKVCache, out: torch.Tensor, 
         tensors += (ks, vs)
     lam_ptr, lam_t, lam_h, lam_value, weight = 0, 0, 0, 0.0, 0
     if maps == 2:
+        if norm and not eps > 0:
+            raise ValueError("eps must be positive: a row without keys is all zeros")
+        if lam is None:
+            raise ValueError("lam must be a float or an fp32 tensor")
         if isinstance(lam, torch.Tensor):
             if lam.dtype != torch.float32 or lam.dim() > 2:
                 raise ValueError("lam must be fp32: one value, [pairs] or [rows, pairs]")

@@ -56,7 +56,7 @@ class Case:
 
 
 def make(lens, new=None, *, heads=8, kv_heads=2, dim=64, page=16, kv="fp16", io=None, maps=1, seed=0, spare=3,
-         interleaved=False, table_extra=2, norm=True, weight=True, lam="heads", v_mean=0.0, device="cuda"):
+         interleaved=False, table_extra=2, norm=True, weight=True, lam="heads", v_mean=0.0, scaled=True, device="cuda"):
     """A seeded case; ``new`` None makes it single-token.  Heads are counted in pairs for maps = 2.
 
     Everything the operators must not read is poisoned: tokens behind a request's length and pages
@@ -87,7 +87,7 @@ def make(lens, new=None, *, heads=8, kv_heads=2, dim=64, page=16, kv="fp16", io=
             x.view(torch.uint8 if x.element_size() == 1 else torch.int16)[dead] = 0x7F if x.element_size() == 1 else 0x7FFF
         ten.append(x)
     scales = [None, None]
-    if kv in ("int8", "fp8_e5m2"):
+    if kv == "int8" or (kv == "fp8_e5m2" and scaled):
         for i in range(2):
             s = torch.randn(pool, page, kv_heads, generator=gen).abs() / 127 + 1e-4 if kv == "int8" else \
                 torch.rand(pool, page, kv_heads, generator=gen) * 1.5 + 0.5

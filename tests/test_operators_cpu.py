@@ -98,7 +98,7 @@ def test_prefill_refuses(break_it):
 
 @pytest.mark.parametrize("more", [dict(lam=torch.zeros(3)), dict(lam=torch.zeros(4).double()), dict(lam=torch.zeros(1, 2, 4)),
                                   dict(norm_weight=torch.zeros(64)), dict(norm_weight=torch.zeros(128).half()),
-                                  dict(norm=False), dict(kernel="fast"), dict(status=torch.zeros(1)),
+                                  dict(norm=False), dict(eps=0.0), dict(eps=-1e-5), dict(lam=None), dict(kernel="fast"), dict(status=torch.zeros(1)),
                                   dict(out=torch.empty(12, 4, 64, dtype=torch.float16)),
                                   dict(out=torch.empty(12, 4, 128, dtype=torch.bfloat16))])
 def test_differential_arguments_refused(more):
@@ -136,7 +136,7 @@ def test_c_entries_check_for_themselves():
     for kw in (dict(q=0), dict(out=0), dict(k_cache=0), dict(block_table=0), dict(seq_lens=0), dict(num_rows=-1), dict(batch=-1),
                dict(num_q_heads=3), dict(num_kv_heads=0), dict(maps=3), dict(maps=2, num_kv_heads=1), dict(block_size=0),
                dict(num_blocks=0), dict(max_blocks_per_seq=0), dict(kv_dtype=4), dict(kv_dtype=3), dict(io_dtype=2), dict(kernel=3),
-               dict(max_seq_len=-1), dict(k_scale=16), dict(block_table_stride=0), dict(query_start=0)):
+               dict(max_seq_len=-1), dict(maps=2, norm=1, eps=0.0), dict(k_scale=16), dict(block_table_stride=0), dict(query_start=0)):
         assert rc(**kw) == -1, kw
     for kw in (dict(head_dim=96), dict(kv_stride_token=100), dict(k_cache=8)):
         assert rc(**kw) == -2, kw

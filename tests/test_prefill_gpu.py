@@ -210,12 +210,43 @@ def test_prefill_sm_scale_and_layouts():
     ref.check(c.call(), c, "odd", r)
 
 
-def test_prefill_large_scores():
+@pytest.mark.parametrize("kv", ["fp16", "bf16", "int8", "fp8_e5m2"])
+def test_prefill_large_scores(kv):
     """Scores of some hundreds: the running maximum moves, probabilities underflow."""
     for maps in (1, 2):
-        c = ref.make([700], [400], heads=2, kv_heads=1, dim=64, maps=maps, norm=False)
+        c = ref.make([700], [400], heads=2, kv_heads=1, dim=64, kv=kv, maps=maps, norm=False)
         c.q *= 16
         both(c)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_unscaled_fp8_pages(dim):
+    for maps in (1, 2):
+        both(ref.make([1, 17, 200, 300], [1, 17, 3, 129], heads=4, kv_heads=2, dim=dim, kv="fp8_e5m2", scaled=False, maps=maps), "stream")
+    both(ref.make([1, 17, 0, 333], heads=4, kv_heads=2, dim=dim, kv="fp8_e5m2", scaled=False, maps=2), "stream")
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+def test_prefill_many_requests(maps):
+    """More requests than one probe of 32 finds, some without rows or keys."""
+    lens = [(i * 7) % 23 for i in range(1100)]
+    new = [n if i % 3 else min(n, 1) for i, n in enumerate(lens)]
+    both(ref.make(lens, new, heads=2, kv_heads=1, dim=64, maps=maps), "stream")
+
+
+@pytest.mark.parametrize("kv", ["fp16", "int8"])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_prefill_split_contexts_of_different_lengths(maps, kv):
+    """Few rows and long keys: the keys are split, the short request has fewer pieces than there are splits."""
+    both(ref.make([20000, 130, 7000, 0], [3, 4, 130, 0], heads=4, kv_heads=2, dim=128, kv=kv, maps=maps), "stream")
+
+
+def test_out_may_be_q():
+    c = ref.make([300, 40], [200, 40], heads=4, kv_heads=2, dim=64)
+    r = ref.reference(c)
+    q = c.q
+    c.q = q.clone()
+    ref.check(c.call(out=c.q), c, "in place", r)
 
 
 def test_empty_calls():
