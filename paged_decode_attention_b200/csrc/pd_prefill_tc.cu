@@ -32,40 +32,61 @@ __global__ void __launch_bounds__(128) tc_join_kernel(const TcParams tp, const i
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) {
     const int64_t first = ((int64_t)row * heads + hq) * MAPS + i, step = (int64_t)a.rows * heads * MAPS;
+    // lane l has the weights of splits l and l + 32
+    float w[2];
     float top = -INFINITY;
-    for (int s = lane; s < tp.splits; s += 32) top = fmaxf(top, __ldg(tp.part_lse + first + s * step));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int s = lane + 32 * k;
+      w[k] = s < tp.splits ? __ldg(tp.part_lse + first + s * step) : -INFINITY;
+      top = fmaxf(top, w[k]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-    float total = 0.f;
+    const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) w[k] = exp2f(w[k] - from);
+    float total = w[0] + w[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[i][e] = 0.f;
-    if (top > -INFINITY) {
-      for (int s = 0; s < tp.splits; ++s) {
-        const float lse = __ldg(tp.part_lse + first + s * step);
-        if (lse == -INFINITY) continue;  // an empty split wrote no row
-        const float w = exp2f(lse - top);
-        total += w;
+    // four splits' rows in flight at a time (one after the other 18 splits took 12 us, most of it waiting)
+    for (int s0 = 0; s0 < tp.splits; s0 += 4) {
+      float y[4][PER], u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int s = s0 + k;
+        u[k] = __shfl_sync(kFull, s & 32 ? w[1] : w[0], s & 31);  // beyond the last split: lane 63's and so on, zero
         const float* src = tp.part_o + (first + s * step) * W;
 #pragma unroll
         for (int e = 0; e < PER; e += RUN) {
           const float* at = src + (e / RUN) * 32 * RUN + lane * RUN;
-          if constexpr (RUN == 4) {
-            const float4 y = __ldg(reinterpret_cast<const float4*>(at));
-            x[i][e] = fmaf(w, y.x, x[i][e]);
-            x[i][e + 1] = fmaf(w, y.y, x[i][e + 1]);
-            x[i][e + 2] = fmaf(w, y.z, x[i][e + 2]);
-            x[i][e + 3] = fmaf(w, y.w, x[i][e + 3]);
-          } else {
-            const float2 y = __ldg(reinterpret_cast<const float2*>(at));
-            x[i][e] = fmaf(w, y.x, x[i][e]);
-            x[i][e + 1] = fmaf(w, y.y, x[i][e + 1]);
+#pragma unroll
+          for (int q = 0; q < RUN; ++q) y[k][e + q] = 0.f;
+          if (u[k] != 0.f) {  // an empty split wrote no row
+            if constexpr (RUN == 4) {
+              const float4 z = __ldg(reinterpret_cast<const float4*>(at));
+              y[k][e] = z.x;
+              y[k][e + 1] = z.y;
+              y[k][e + 2] = z.z;
+              y[k][e + 3] = z.w;
+            } else {
+              const float2 z = __ldg(reinterpret_cast<const float2*>(at));
+              y[k][e] = z.x;
+              y[k][e + 1] = z.y;
+            }
           }
         }
       }
-      const float inv = 1.f / total;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) x[i][e] *= inv;
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[i][e] = fmaf(u[k], y[k][e], x[i][e]);
     }
+    const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x[i][e] *= inv;
   }
   float factor = 1.f;
   if constexpr (MAPS == 2) {
