@@ -13,6 +13,9 @@
 // takes the block id from the free list itself, so nobody waits for the row being written.  The
 // cluster barrier stands between the last read of the lengths and of num_free and their first
 // write, which is what lets a caller update them in place without a counter in memory.
+//
+// 256 requests with a token each: 7.4 us a launch in a graph; 64 requests, 64 k tokens: 7.0 us; an empty launch
+// takes 2 to 3.  The rest is the chain lengths -> scan -> block id -> store of dependent memory accesses.
 #include "pd_common.cuh"
 
 namespace pd {

@@ -25,6 +25,12 @@
 // that are no multiple of 16 tokens come by 16-byte asynchronous copies, row by row.  V's rows behind the last
 // key are cleared behind the copy, because zero times the NaN that a page may hold would stay.
 //
+// P is rounded to the pages' 16-bit type for the product with V: relative to a result about what rounding
+// the result itself costs (2.1e-4 of its norm in fp16, 1.7e-3 in bf16).  The difference of two maps that share
+// V has sqrt((1 + lambda^2) / (1 + lambda^2 - 2 lambda r)) times as much, r their overlap: 3.2e-4 in all for
+// fp16.  A second 16-bit term of the first map's P (products with V and stores of P half as many again) brought
+// that to 2.3e-4 and cost 14 to 21 % (4096 new tokens of 16/4 heads, head_dim 128, fp16: 290 -> 350 us).
+//
 // The maximum that P refers to may lag behind the true one by kLag (2^3 or 2^8 at most): O is then not
 // rescaled for every small rise.  It cancels in O / l; l and O are 32-bit.
 //
@@ -33,7 +39,12 @@
 //
 // 8-bit pages: four more warps read the pages, widen the elements exactly and store them in the
 // same swizzle; K's scales multiply S, V's scales multiply P (times 32, against fp16's subnormals),
-// so nothing is rounded on the way.
+// so nothing is rounded on the way.  Six chunks of 100 to 512 tokens behind 1 to 16 k of int8 keys (28/4 heads,
+// head_dim 128): 201 us, 470 TFLOP/s; the scales' two multiplications a score on the softmax warps bound it.
+//
+// Two maps: one prompt of 4096 tokens, 16/4 pairs of head_dim 128, fp16: 290 us, 710 TFLOP/s, a third of the
+// products more than counted because both CTAs of a cluster need S.  Drafts of 3 to 5 tokens behind 16 to 32 k
+// (16/4 pairs of 64): 59 us, 3.3 TB/s, split 18 ways; the number of TMA boxes and the join bound it.
 //
 // Every wait is bounded; one that gives up raises PD_DEV_TIMEOUT and ends the CTA's loops.  Nobody
 // skips a barrier on that way, tensor memory is freed, and copies and products in flight are
