@@ -229,7 +229,8 @@ extern "C" PD_API int pd_plan_step(const PdPlanArgs* a) {
   int ctas = 1;
   while (ctas < kPlanMaxCtas && (int64_t)ctas * kPlanThreads * (few ? 1 : kPlanRunMany) < a->num_tokens) ctas <<= 1;
   const size_t smem = (size_t)(a->batch + 1) * sizeof(PlanRow);
-  if (smem > 48 * 1024 &&
+  // 48 KB are granted unasked, to the rows here and the kernel's static arrays (some 150 bytes) together
+  if (smem > 47 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            (int)((kPlanMaxBatch + 1) * sizeof(PlanRow))) != cudaSuccess)
     return PD_ERR_CUDA;
