@@ -337,8 +337,10 @@ PD_API int pd_cache_write(const PdCacheWriteArgs* args);
  * [query_start[b], query_start[b + 1]) of q and out, and they are the LAST tokens of its
  * seq_lens[b] cached tokens (write them with pd_cache_write first).  The token at position p of a
  * request attends to its keys 0 .. p.  Rows of q beyond query_start[batch] belong to nobody: their
- * rows of out are left as they were.  A row whose position is below zero (more query rows than
- * cached tokens) attends to nothing and gives zeros.
+ * rows of out are left as they were.  Where query_start names more rows than num_rows, those from
+ * num_rows on are cut off: nothing is computed for them, the others keep their positions.  A row
+ * whose position is below zero (more query rows than cached tokens) attends to nothing and gives
+ * zeros.
  *
  * maps = 1: out[t, h] = softmax(q[t, h] K^T * sm_scale) V.
  * maps = 2 (differential): kv heads 2j and 2j + 1 are the two keys of pair j and their value rows,

@@ -367,14 +367,14 @@ __device__ __forceinline__ bool tc_find_tile(const PrefillParams& a, int rows_pe
     n = min(step, n - k * step);
   }
   const int start = __ldg(a.starts + lo);
-  int tokens = __ldg(a.starts + lo + 1) - start;
+  const int tokens = __ldg(a.starts + lo + 1) - start;
   if (start < 0 || start >= a.rows || tokens <= 0) return false;
-  tokens = min(tokens, a.rows - start);
+  const int held = min(tokens, a.rows - start);  // of them in q; those cut off still count for the others' positions
   const int64_t local = i - ((int64_t)start * group / rows_per_tile + lo);
-  if (local < 0 || local * rows_per_tile >= (int64_t)tokens * group) return false;
+  if (local < 0 || local * rows_per_tile >= (int64_t)held * group) return false;
   t.request = lo;
   t.row0 = (int)(local * rows_per_tile);
-  t.count = (int)min((int64_t)rows_per_tile, (int64_t)tokens * group - t.row0);
+  t.count = (int)min((int64_t)rows_per_tile, (int64_t)held * group - t.row0);
   t.first_token = start;
   t.tokens = tokens;
   t.len = clamp_len(p, lo);

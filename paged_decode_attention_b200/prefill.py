@@ -182,7 +182,8 @@ def paged_prefill(q: torch.Tensor, cache: PagedKVCache, query_start_loc: torch.T
 
     Request b owns the rows ``query_start_loc[b] : query_start_loc[b + 1]`` (int32 ``[B + 1]``); they are
     the last of its ``cache.seq_lens[b]`` cached tokens, and each attends to the keys up to its own
-    position.  Rows behind ``query_start_loc[B]`` are left as they were in ``out``; a request with more
+    position.  Rows behind ``query_start_loc[B]`` are left as they were in ``out``; rows that it names behind
+    the last of q are cut off, and the others keep their positions; a request with more
     rows than cached tokens has rows that attend to nothing, which are zero.  ``max_seq_len`` is an
     optional host-side bound on ``seq_lens`` that refines how long contexts of few rows are split.
     ``kernel`` and ``status`` are as for ``paged_decode``.
