@@ -1520,7 +1520,10 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
             if (gq == 0) p.res_lse[(int64_t)vi.b * p.hq + hq] = lse;
           }
         } else {
-          const int64_t slot_row = (int64_t)(w + v) * hg + role * p.group + head;
+          // w + v names one segment where both grow along the tile line.  Requests dealt whole (they write
+          // partials only in pairs) go to the workers in another order, and one has no more than v itself.
+          const int slot = MAPS == 2 && dealt_whole ? v : w + v;
+          const int64_t slot_row = (int64_t)slot * hg + role * p.group + head;
           dst32 = p.part_o + slot_row * (MAPS * D);
           if (gq == 0) p.part_lse[slot_row] = lse;
         }
@@ -1587,8 +1590,7 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
       // request run on different SMs at the same time.
       int wfirst = 0, nseg = 0;
       if (MAPS == 2 && dealt_whole) {
-        wfirst = w;  // the pair's two warps are in this worker; there is no boundary table
-        nseg = 1;
+        nseg = 1;  // the pair's two warps are in this worker, its slot is v0; there is no boundary table
       } else if (sp.splits == 1) {
         wfirst = cm.of(prefix[v0]);
         nseg = cm.of(prefix[v0 + 1] - 1) - wfirst + 1;

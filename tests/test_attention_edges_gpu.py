@@ -3,10 +3,13 @@ the definitions in 64 bits, with the bounds derived in operators_ref."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import operators_ref as ref
+from paged_decode_attention_b200 import _cabi, prefill as pre
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +32,27 @@ def test_rows_are_cut_off_where_the_starts_name_more(kernel, maps, kv, lens, new
     r = ref.reference(c)
     c.q = c.q[:rows].contiguous()
     check_rows(c.call(kernel=kernel), c, r, rows, kernel)
+
+
+@pytest.mark.parametrize("kv", ["fp16", "int8"])
+@pytest.mark.parametrize("kv_heads", [1, 2, 4])
+@pytest.mark.parametrize("sm_count,requests", [(2, 3), (2, 4), (5, 10), (8, 9), (140, 141), (140, 280), (148, 296)])
+def test_short_requests_dealt_whole_to_any_number_of_sms(sm_count, requests, kv_heads, kv):
+    """Fewer requests than workers, none longer than 256 tokens, no room in the table for longer ones: each worker
+    has one, and the two maps of a pair meet in scratch rows that nobody else may touch."""
+    c = ref.make([96 + 7 * (i % 5) for i in range(requests)], heads=2 * kv_heads, kv_heads=kv_heads, dim=64, kv=kv, maps=2,
+                 seed=requests)
+    r = ref.reference(c)
+    out = torch.empty(requests, c.q.shape[1], 128, dtype=c.q.dtype, device="cuda")
+    lib, need = _cabi.load(), ctypes.c_uint64(0)
+    values = pre.build_prefill_args(c.q, c.cache, out, None, maps=2, lam=c.lam, kernel="stream", sm_count=sm_count,
+                                    stream=torch.cuda.current_stream().cuda_stream, **c.kwargs())
+    names = [n for n, _ in _cabi.PdPrefillArgs._fields_]
+    _cabi.check(lib.pd_prefill_workspace_bytes(pre._PACK.pack(*values), ctypes.byref(need)), "pd_prefill_workspace_bytes")
+    scratch = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    values[names.index("workspace")], values[names.index("workspace_bytes")] = scratch.data_ptr(), need.value
+    block = pre._PACK.pack(*values)
+    for _ in range(30):
+        out.fill_(float("nan"))
+        _cabi.check(lib.pd_diff_decode(block), "pd_diff_decode")
+        check_rows(out, c, r, requests)
