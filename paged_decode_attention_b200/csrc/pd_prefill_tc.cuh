@@ -866,7 +866,9 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
     const int n_rows = rows_of[t];
 
     // ---- Q into shared memory, 16 bytes at a time, in the 128-byte swizzle --------------------------
-    if (jend > j0) {
+    // Not for a tile whose rows all see nothing beside one that has keys: no product reads it, so nothing would
+    // stand between these copies, which land all over the tile, and the zero results that pass through it.
+    if (end[t] > j0) {
       constexpr int CH = D / 8;         // 16-byte chunks of a row
       constexpr int RPI = 128 / CH;     // rows of one round of the tile's threads
       const int c = me % CH, rr = me / CH;
@@ -886,8 +888,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async();
-      mbar_arrive(q_full);
     }
+    if (jend > j0) mbar_arrive(q_full);
 
     const int limit = me < n_rows ? tc_limit(tile, first_row + me, p.group) : 0;
     const int least = n_rows ? tc_limit(tile, first_row, p.group) : 0;  // the tile's row that sees the fewest

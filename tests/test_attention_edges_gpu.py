@@ -56,3 +56,23 @@ def test_short_requests_dealt_whole_to_any_number_of_sms(sm_count, requests, kv_
         out.fill_(float("nan"))
         _cabi.check(lib.pd_diff_decode(block), "pd_diff_decode")
         check_rows(out, c, r, requests)
+
+
+@pytest.mark.parametrize("kernel", ["simple", "stream"])
+@pytest.mark.parametrize("kv", ["fp16", "bf16", "int8", "fp8_e5m2"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cached,new", [(100, 200), (40, 101), (1, 64), (200, 300)])
+def test_many_rows_without_keys_beside_rows_with_keys(kernel, kv, dim, cached, new):
+    """More new tokens than cached ones, by so many that 128 packed rows and more attend to nothing while others of
+    their CTA have keys: those rows are zeros in every call."""
+    batch = 40
+    c = ref.make([cached] * batch, [new] * batch, heads=8, kv_heads=2, dim=dim, kv=kv, seed=new)
+    r = ref.reference(c)
+    empty = (torch.arange(new, device="cuda") < new - cached).repeat(batch)
+    assert int(empty.sum()) * 4 // batch >= 128 and (r[0][empty] == 0).all()
+    out = torch.empty(c.q.shape, dtype=c.q.dtype, device="cuda")
+    for _ in range(1 if kernel == "simple" else 20):
+        out.fill_(float("nan"))
+        c.call(out=out, kernel=kernel)
+        assert (out[empty] == 0).all()
+        check_rows(out, c, r, batch * new, kernel)
