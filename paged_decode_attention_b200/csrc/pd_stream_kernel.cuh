@@ -1280,10 +1280,6 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     int j = g - prefix[v];
     const bool whole = MAPS == 1 && (j == 0) && (seg_end == vend) && (sp.splits == 1) && !pushing;
     const int kvh = vi.hb * HB + role;
-    // first query row of this kv head's group and the stride between the rows; the heads of a
-    // pair alternate in the cache (MAPS = 2), their query rows are q_sm apart
-    const int64_t q_first = MAPS == 2 ? (int64_t)(kvh >> 1) * p.group * p.q_sh + (kvh & 1) * sp.diff.q_sm
-                                      : (int64_t)kvh * p.group * p.q_sh;
 
     // ---- query rows of this kv head's group as B fragments: thread (g, t) holds head g (+8 per
     // n-tile), head_dim pairs of its k slots; heads >= group are zero --------------------------
@@ -1334,7 +1330,12 @@ stream_decode_kernel(const __grid_constant__ StreamParams sp, const __grid_const
     if (qstage) {
       fill_fragments([&](int head, int col) { return lds32(qstage + (uint32_t)head * kQPitch + 2u * (uint32_t)col); });
     } else {
-      const __half* qrows = (const __half*)p.q + (int64_t)vi.b * p.q_sb + q_first;
+      // the heads of a pair alternate in the cache (MAPS = 2), their query rows are q_sm apart.  (Computed here:
+      // across the staging branch it cost plain decode at head_dim 128 spilled registers; 32 requests of 8192, 32/4
+      // heads, scaled e5m2: 61.2 against 60.3 us.)
+      const __half* qrows = (const __half*)p.q + (int64_t)vi.b * p.q_sb +
+                            (MAPS == 2 ? (int64_t)(kvh >> 1) * p.group * p.q_sh + (kvh & 1) * sp.diff.q_sm
+                                       : (int64_t)kvh * p.group * p.q_sh);
       fill_fragments([&](int head, int col) {
         return __ldg(reinterpret_cast<const uint32_t*>(qrows + (int64_t)head * p.q_sh + col));
       });
