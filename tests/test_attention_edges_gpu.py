@@ -4,6 +4,7 @@ the definitions in 64 bits, with the bounds derived in operators_ref."""
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 
 import pytest
 import torch
@@ -76,3 +77,32 @@ def test_many_rows_without_keys_beside_rows_with_keys(kernel, kv, dim, cached, n
         c.call(out=out, kernel=kernel)
         assert (out[empty] == 0).all()
         check_rows(out, c, r, batch * new, kernel)
+
+
+def without_poison(c):
+    """The same case with finite values wherever it has NaN, so that a page left out counts as nothing in the
+    reference: zero times what stands in the page read in its place."""
+    def clean(t):
+        return t if t is None or t.dtype is torch.int8 else torch.nan_to_num(t.float(), 0.0).to(t.dtype)
+
+    tensors = {n: clean(getattr(c.cache, n)) for n in ("k_cache", "v_cache", "k_scale", "v_scale")}
+    return dataclasses.replace(c, cache=dataclasses.replace(c.cache, **tensors))
+
+
+@pytest.mark.parametrize("kernel", ["simple", "stream"])
+@pytest.mark.parametrize("kv", ["fp16", "bf16", "int8", "fp8_e5m2"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("maps,new", [(1, [300, 10, 20, 64]), (2, [300, 10, 20, 64]), (2, None)])
+def test_pages_outside_the_pool_count_as_nothing(kernel, kv, dim, maps, new):
+    """Every row is compared, also those of requests that lose a page, and the one that loses all of them gives zeros."""
+    for seed in range(3):
+        c = ref.make([300, 64, 2500, 64], new, heads=4, kv_heads=2, dim=dim, kv=kv, maps=maps, seed=seed)
+        table = c.cache.block_table
+        table[0, 3], table[1, 0], table[2, 1], table[2, 100] = 10 ** 6, -1, -3, c.cache.num_blocks
+        table[3] = -1
+        r = ref.reference(without_poison(c))
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = c.call(kernel=kernel, status=status)
+        assert int(status) == _cabi.DEV_BAD_BLOCK
+        check_rows(got, c, r, got.shape[0], kernel)
+        assert (got[-(64 if new else 1):] == 0).all()
