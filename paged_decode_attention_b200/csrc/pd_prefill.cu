@@ -87,7 +87,7 @@ static void fill(const PdPrefillArgs* a, PrefillParams& r) {
   r.lam_st = a->lam_stride_t;
   r.lam_sh = a->lam_stride_h;
   r.lam_value = a->lam_value;
-  r.weight = a->norm_weight;
+  r.weight = a->norm ? a->norm_weight : nullptr;  // the weight belongs to the norm
   r.eps = a->eps;
   r.out_scale = a->out_scale;
   r.norm = a->norm;

@@ -395,7 +395,7 @@ int diff_stream_supports(const PdPrefillArgs* a) {
   const int why = stream_supports(&d);
   if (why != PD_OK) return why;
   if (a->q_stride_m % 2) return PD_ERR_UNSUPPORTED;
-  if (a->norm_weight && ((uintptr_t)a->norm_weight % 16)) return PD_ERR_UNSUPPORTED;
+  if (a->norm && a->norm_weight && ((uintptr_t)a->norm_weight % 16)) return PD_ERR_UNSUPPORTED;
   const Shape s = derive(&d, 2);
   SmemPlan sm;
   return plan_smem(s, sm) ? PD_OK : PD_ERR_UNSUPPORTED;
@@ -420,7 +420,7 @@ int diff_stream_run(const PdPrefillArgs* a, int sm_count) {
   t.lam = a->lam;
   t.lam_sb = a->lam_stride_t;
   t.lam_sh = a->lam_stride_h;
-  t.weight = a->norm_weight;
+  t.weight = a->norm ? a->norm_weight : nullptr;  // the weight belongs to the norm
   t.lam_value = a->lam_value;
   t.eps = a->eps;
   t.out_scale = a->out_scale;

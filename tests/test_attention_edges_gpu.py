@@ -106,3 +106,27 @@ def test_pages_outside_the_pool_count_as_nothing(kernel, kv, dim, maps, new):
         assert int(status) == _cabi.DEV_BAD_BLOCK
         check_rows(got, c, r, got.shape[0], kernel)
         assert (got[-(64 if new else 1):] == 0).all()
+
+
+@pytest.mark.parametrize("kernel", ["simple", "stream"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [None, [30, 4], [130, 200]])
+def test_without_the_norm_its_weight_is_not_applied(kernel, dim, new):
+    """The C ABI's formula: a weight that stands in an argument block whose ``norm`` is 0 is no part of the result."""
+    c = ref.make([700, 260], new, heads=4, kv_heads=2, dim=dim, maps=2)
+    kw = c.kwargs()
+    weight = c.weight
+    c.norm, c.weight = False, None
+    r = ref.reference(c)
+    out = torch.full((c.q.shape[0], c.q.shape[1], 2 * dim), float("nan"), dtype=c.q.dtype, device="cuda")
+    lib, need = _cabi.load(), ctypes.c_uint64(0)
+    values = pre.build_prefill_args(c.q, c.cache, out, c.starts, maps=2, lam=c.lam, kernel=kernel,
+                                    stream=torch.cuda.current_stream().cuda_stream, **{**kw, "norm_weight": weight})
+    at = {n: i for i, (n, _) in enumerate(_cabi.PdPrefillArgs._fields_)}
+    values[at["norm"]] = 0
+    _cabi.check(lib.pd_prefill_workspace_bytes(pre._PACK.pack(*values), ctypes.byref(need)), "pd_prefill_workspace_bytes")
+    scratch = torch.empty(max(need.value, 1), dtype=torch.uint8, device="cuda")
+    values[at["workspace"]], values[at["workspace_bytes"]] = scratch.data_ptr(), need.value
+    entry = lib.pd_diff_decode if new is None else lib.pd_prefill
+    _cabi.check(entry(pre._PACK.pack(*values)), "call")
+    check_rows(out, c, r, out.shape[0], kernel)
