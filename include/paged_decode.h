@@ -385,7 +385,7 @@ typedef struct PdPrefillArgs {
   int32_t norm;                /* 0: no norm */
   int32_t kernel;              /* PD_KERNEL_*: STREAM is the one on the matrix units */
   int32_t sm_count;            /* 0 = query the current device */
-  int32_t max_seq_len;         /* optional bound on seq_lens (0 = unknown): refines the split count */
+  int32_t max_seq_len;         /* optional bound on seq_lens (0 = unknown: the table's width): sets the split count */
   void* workspace;             /* 256-byte aligned, pd_prefill_workspace_bytes() bytes */
   uint64_t workspace_bytes;
   uint32_t* status;            /* optional device word, OR-ed with PD_DEV_* bits; caller zeroes it */
@@ -412,7 +412,8 @@ PD_API int pd_prefill_select_kernel(const PdPrefillArgs* args);
  * pages it has.  A request is served if its row has room for all its pages and the free list
  * holds the pages of all such requests up to and including it; one that needs no page always is.
  * A request that is not served keeps its length and its row, its tokens get slot -1, and
- * PD_DEV_NO_BLOCKS is raised.
+ * PD_DEV_NO_BLOCKS is raised.  query_start counts its tokens all the same, so attention over the
+ * step's rows takes them for its last cached tokens: such rows of out mean nothing.
  *
  * Outputs: slot_mapping[t] = block * block_size + offset of new token t (request after request),
  * positions[t] its position in its request; entries behind the last new token are -1 and 0.

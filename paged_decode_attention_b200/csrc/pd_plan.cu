@@ -6,7 +6,7 @@
 // and need_b = 0 or I_b <= num_free; page k of need_b comes from free_blocks[num_free - 1 -
 // (I_b - need_b + k)].  A token's slot is table[b, pos / P] * P + pos % P.
 //
-// Bound by latency: a decode step of 256 requests moves 9 KB, a step of 64 k prompt tokens 1 MB.
+// Bound by latency: a decode step of 256 requests moves 9 KB, a step of 64 requests with 10 k prompt tokens 172 KB.
 // So it is one launch of one thread-block cluster (1 to 8 CTAs).  Every CTA makes the scans over
 // the requests for itself in shared memory (a few microseconds' worth of nothing to exchange
 // otherwise), then the CTAs share out the tokens and the table rows.  A token in a new page
@@ -14,7 +14,7 @@
 // cluster barrier stands between the last read of the lengths and of num_free and their first
 // write, which is what lets a caller update them in place without a counter in memory.
 //
-// 256 requests with a token each: 7.4 us a launch in a graph; 64 requests, 64 k tokens: 7.0 us; an empty launch
+// 256 requests with a token each: 7.3 us a launch in a graph; 64 requests, 10479 tokens: 6.8 us; an empty launch
 // takes 2 to 3.  The rest is the chain lengths -> scan -> block id -> store of dependent memory accesses.
 #include "pd_common.cuh"
 

@@ -137,8 +137,12 @@ static TcPlan tc_plan(const PdPrefillArgs* a, int sm_count) {
   // Up to half a wave of tiles: pieces for one wave, of kTcLeast blocks and more, with room for twice as many
   // pieces of a context as of the mean one.  Up to two waves: pieces for three waves, of at least kTcLong blocks,
   // because contexts of a batch differ and the last tile to end is a long one; shorter pieces cost more in
-  // starts and in the join than they even out (2048 tokens of 32/8 heads, 264 tiles: 56 us, in two pieces
-  // 100 us).  Beyond, the order of the tiles evens it out.
+  // starts and in the join than they even out (2048 tokens of 32/8 heads, 264 tiles: 47 us whole, 92 in two
+  // pieces).  Beyond, the order of the tiles evens it out.
+  // The lengths themselves are on the device.  What is known here is the room in the block table, or the
+  // caller's max_seq_len where that is less: with a table wider than the contexts and no max_seq_len, contexts
+  // too short for it are cut as well, into pieces of kTcLeast blocks and more, and all rows go through the join
+  // (tables of 32768 tokens: 512 tokens of 32/8 heads 17 -> 29 us, the 2048 above 47 -> 92; with max_seq_len as exact).
   int64_t bound = (int64_t)a->max_blocks_per_seq * a->block_size;
   if (a->max_seq_len > 0 && a->max_seq_len < bound) bound = a->max_seq_len;
   const int64_t ctas = (int64_t)t.tiles * t.heads * s.slices;

@@ -20,9 +20,9 @@
 //
 // Three warps fill the ring, a lane for each TMA box of up to 128 tokens of a page and 64 columns.  What
 // such boxes cost is their number: 32 of 16 tokens a block keep pace with the products only when the waits
-// leave the SM alone and several warps issue (8192 tokens of 32/8 heads, head_dim 128, bf16: 456 us at
-// pages of 16 and of 128 alike, 1.2 PFLOP/s; one loader and polling waits: 649).  Pages
-// that are no multiple of 16 tokens come by 16-byte asynchronous copies, row by row.  V's rows behind the last
+// leave the SM alone and several warps issue (8192 tokens of 32/8 heads, head_dim 128, bf16, one set of inputs in a
+// graph: 457 us at pages of 16 and of 128 alike, 1.2 PFLOP/s; one loader and polling waits: 649.  Calls over changing
+// inputs under the power cap: 534, 1.03 PFLOP/s).  Pages that are no multiple of 16 tokens come by 16-byte asynchronous copies, row by row.  V's rows behind the last
 // key are cleared behind the copy, because zero times the NaN that a page may hold would stay.
 //
 // P is rounded to the pages' 16-bit type for the product with V: relative to a result about what rounding
@@ -39,12 +39,14 @@
 //
 // 8-bit pages: four more warps read the pages, widen the elements exactly and store them in the
 // same swizzle; K's scales multiply S, V's scales multiply P (times 32, against fp16's subnormals),
-// so nothing is rounded on the way.  Six chunks of 100 to 512 tokens behind 1 to 16 k of int8 keys (28/4 heads,
-// head_dim 128): 201 us, 470 TFLOP/s; the scales' two multiplications a score on the softmax warps bound it.
+// so nothing is rounded on the way but P itself; its sum l is that of the unrounded P, as P is rounded once for
+// each value head, with that head's scales.  32 P times the scale keeps fp16's 11 bits
+// down to 2^-14, below that it has a step of 2^-24.  Six chunks of 159 to 503 tokens behind 1.8 to 5.3 k of int8 keys (28/4 heads,
+// head_dim 128): 201 us, 475 TFLOP/s; the scales' two multiplications a score on the softmax warps bound it.
 //
-// Two maps: one prompt of 4096 tokens, 16/4 pairs of head_dim 128, fp16: 290 us, 710 TFLOP/s, a third of the
-// products more than counted because both CTAs of a cluster need S.  Drafts of 3 to 5 tokens behind 16 to 32 k
-// (16/4 pairs of 64): 59 us, 3.3 TB/s, split 18 ways; the number of TMA boxes and the join bound it.
+// Two maps: one prompt of 4096 tokens, 16/4 pairs of head_dim 128, fp16: 292 us, 706 TFLOP/s, a third of the
+// products more than counted because both CTAs of a cluster need S.  Drafts of 4 or 5 tokens behind 22 to 25 k
+// (16/4 pairs of 64): 60 us, 3.3 TB/s, split 18 ways; the number of TMA boxes and the join bound it.
 //
 // Every wait is bounded; one that gives up raises PD_DEV_TIMEOUT and ends the CTA's loops.  Nobody
 // skips a barrier on that way, tensor memory is freed, and copies and products in flight are
@@ -981,7 +983,8 @@ tc_prefill_kernel(const __grid_constant__ TcParams tp, const __grid_constant__ C
             for (int c = 0; c < 32; c += 2) {
               pk[c / 2] = tc_pack<C::BF16>(y[c], y[c + 1]);
               // For a pair l is the sum of what the product with V reads, the rounded probabilities: what their
-              // roundings have in common then cancels in O / l, which the difference of the two maps needs.
+              // roundings have in common then cancels in O / l (700 new tokens, values with a mean of one standard
+              // deviation, fp16: 2.28e-4 -> 2.21e-4 of the result; values without a mean: no difference).
               if constexpr (MAPS == 2) add_pair<C::BF16>(sum[c & 2], sum[(c & 2) + 1], pk[c / 2]);
             }
           }

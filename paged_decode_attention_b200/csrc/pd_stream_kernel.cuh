@@ -382,8 +382,8 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
 // are the rows of both heads of its pair side by side (`second` tells which of the two this warp
 // has), so O^T has 2 * D rows; 8-bit pages scale P by each V head's own scale, hence two P^T.
 // Per pair the cache is read once, and a tile of V twice from shared memory.  16/4 pairs of 128: 64 requests
-// of 2 to 8 k in fp16 187 us, 6.2 TB/s; two of 131072 in scaled e5m2 127 us, 4.3 TB/s; 32/4 pairs, 32 requests
-// of 1 to 4 k in int8 67 us, 2.3 TB/s.  8-bit pages are bound by the consumer warps' chain of conversion, softmax
+// of 2 to 8 k in fp16 188 us, 6.1 TB/s; two of 131072 in scaled e5m2 126 us, 4.3 TB/s; 32/4 pairs, 32 requests
+// of 1 to 4 k in int8 65 us, 2.4 TB/s.  8-bit pages are bound by the consumer warps' chain of conversion, softmax
 // and the second product, not by memory.
 template <int KV, int D, int HB, bool SCALED, int NG, bool MASKED, int NT = 1, int MAPS = 1>
 __device__ __forceinline__ void consume_tile(
@@ -580,7 +580,8 @@ __device__ __forceinline__ void consume_tile(
         const uint32_t hi = SCALED ? pack_io2<KV>(p2 * vs[z][u][1], p3 * vs[z][u][1]) : pack_io2<KV>(p2, p3);
         if constexpr (MAPS == 2 && !SCALED) {
           // the sum of the rounded probabilities, as the product reads them: what their roundings have in
-          // common cancels in O / l, which the difference of the two maps needs
+          // common cancels in O / l (0.3 % of the error where values have a mean; scaled pages, whose P is
+          // rounded for each V head's scales apart, sum the unrounded)
           add_pair<KV == PD_KV_BF16>(sum0, sum1, lo);
           add_pair<KV == PD_KV_BF16>(sum0, sum1, hi);
         }

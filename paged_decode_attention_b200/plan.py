@@ -8,7 +8,6 @@ read back to the host, so a step (or a captured graph of steps) needs no synchro
 
 from __future__ import annotations
 
-import ctypes
 import typing
 
 import torch
@@ -57,7 +56,9 @@ def plan_step(block_table: torch.Tensor, context_lens: torch.Tensor, new_tokens:
     changed).  A request is served when its row has room for all its pages and the stack holds the
     pages of all such requests up to and including it (or it needs none); one that is not served
     keeps its length and row, its tokens get slot -1, and ``status`` (an int32 word) gets
-    ``DEV_NO_BLOCKS``.  Block ids are taken as they are; ``cache_write`` and the attention kernels
+    ``DEV_NO_BLOCKS``.  ``query_start_loc`` counts its tokens all the same (their rows of the batch stay
+    where they are), so an attention call of the same step takes them for the last of the cached ones and
+    what it gives for them means nothing: read ``status`` before the results are used.  Block ids are taken as they are; ``cache_write`` and the attention kernels
     check them.
 
     ``out`` receives the results in buffers of the caller, for captured graphs: ``out.seq_lens`` may
